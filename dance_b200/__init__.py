@@ -12,12 +12,12 @@ import ctypes
 import os
 from pathlib import Path
 
-__all__ = ["lib", "load", "LIB_PATH", "DanceError", "DANCE_U8", "DANCE_F16", "DANCE_F32",
+__all__ = ["lib", "load", "LIB_PATH", "DanceError", "DANCE_U8", "DANCE_F16", "DANCE_F32", "DANCE_BF16",
            "DanceVamanaParams", "GPUVamanaStats"]
 
 LIB_PATH = Path(__file__).resolve().parent / "libdance_b200.so"
 
-DANCE_U8, DANCE_F16, DANCE_F32 = 0, 1, 2
+DANCE_U8, DANCE_F16, DANCE_F32, DANCE_BF16 = 0, 1, 2, 3
 
 
 class DanceError(RuntimeError):
@@ -133,6 +133,25 @@ class DanceStitchedStats(ctypes.Structure):
         return {k: getattr(self, k) for k, _ in self._fields_ if not k.startswith("reserved")}
 
 
+class DanceKvCache(ctypes.Structure):
+    """Mirror of ``DanceKvCache`` in include/dance_b200.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_k", "d_v", "d_k_scale", "d_v_scale", "d_k_bounds")] + [
+        (n, ctypes.c_uint64) for n in ("k_block_stride", "v_block_stride")] + [
+        (n, ctypes.c_uint32) for n in ("num_blocks", "kv_heads", "block_tokens", "head_dim")]
+
+
+class DanceKvBatch(ctypes.Structure):
+    """Mirror of ``DanceKvBatch`` in include/dance_b200.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_block_table", "d_seq_lens", "d_row_offsets")] + [
+        (n, ctypes.c_uint32) for n in ("table_width", "batch", "max_rows", "max_len")]
+
+
+class DanceKvRows(ctypes.Structure):
+    """Mirror of ``DanceKvRows`` in include/dance_b200.h."""
+    _fields_ = [("d_data", ctypes.c_void_p), ("row_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64),
+                ("rows", ctypes.c_uint32), ("dtype", ctypes.c_int)]
+
+
 _P = ctypes.c_void_p
 _U32 = ctypes.c_uint32
 _U64 = ctypes.c_uint64
@@ -203,6 +222,12 @@ SIGNATURES = {
     "dance_kmeans_lloyd": (_I, [_P, _U64, _U64, _U32, _U32, _U32, _P, _P, ctypes.POINTER(ctypes.c_double), _P]),
     "dance_partition_assign": (_I, [_I, _P, _U64, _U64, _U32, _P, _U32, _U32, _P, _P, _P]),
     "dance_partition_buckets": (_I, [_P, _U64, _U32, _U32, _P, _P, _P]),
+    "dance_kv_append": (_I, [_P, _P, _P, _P, _P]),
+    "dance_kv_read": (_I, [_P, _P, _U32, _I, _P, _P, _P]),
+    "dance_kv_attention": (_I, [_P, _P, _P, _U32, _F, _P, _P, _P, _U64, _P]),
+    "dance_kv_select_blocks": (_I, [_P, _P, _P, _U32, _U32, _U32, _U32, _P, _P, _U64, _P]),
+    "dance_kv_sparse_attention": (_I, [_P, _P, _P, _U32, _P, _U32, _F, _P, _P, _P, _U64, _P]),
+    "dance_kv_workspace_bytes": (_U64, [_P, _P, _U32, _U32, _U32]),
     "dance_stitched_build_sharded": (_I, [_P, _I, _P, _U32, _U32, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32, _P,
                                           _U32, _P, _P, _U64, _P, _P]),
     "dance_stitched_global_prune": (_I, [_I, _P, _U64, _U32, _U32, _P, _P, _P, _P, _U32, _U32, _F, _P, _P, _P,

@@ -1,6 +1,6 @@
 // host_common.cuh -- host-side plumbing shared by the single-GPU build
-// (vamana_build.cu) and the NCCL-sharded build (vamana_sharded.cu): error
-// reporting, device buffers, dtype/width dispatch, kernel launchers, the
+// (vamana_build.cu) and the NCCL-sharded build (vamana_sharded.cu): device
+// buffers, dtype/width dispatch, kernel launchers, the
 // per-build workspace and the reverse-CSR + merge driver.
 #pragma once
 
@@ -8,8 +8,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
-#include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -18,6 +16,7 @@
 #include "../../include/dance_b200.h"
 #include "../../include/gpu_vamana_builder.h"
 #include "../../include/gpu_vamana_config.h"
+#include "host_errors.cuh"
 #include "vamana_kernels.cuh"
 #include "gram_u8.cuh"
 #include "prune_quad.cuh"
@@ -26,39 +25,7 @@
 namespace dance
 {
 
-// ---------------------------------------------------------------- errors
-extern thread_local char g_err[512];
-extern std::atomic<uint64_t> g_launches;
 extern thread_local DanceBuildReport g_report; // last resident or sharded build
-
-inline int fail(int code, const char *fmt, ...)
-{
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof(g_err), fmt, ap);
-    va_end(ap);
-    fprintf(stderr, "[dance_b200] %s\n", g_err);
-    return code;
-}
-
-#define DANCE_CUDA(call)                                                                                        \
-    do                                                                                                          \
-    {                                                                                                           \
-        cudaError_t e__ = (call);                                                                               \
-        if (e__ != cudaSuccess)                                                                                 \
-            return fail(-2, "CUDA error %s at %s:%d (%s)", cudaGetErrorString(e__), __FILE__, __LINE__, #call); \
-    } while (0)
-
-#define DANCE_LAUNCHED()                                                                                        \
-    do                                                                                                          \
-    {                                                                                                           \
-        g_launches.fetch_add(1, std::memory_order_relaxed);                                                    \
-        cudaError_t e__ = cudaGetLastError();                                                                   \
-        if (e__ != cudaSuccess)                                                                                 \
-            return fail(-2, "kernel launch failed: %s at %s:%d", cudaGetErrorString(e__), __FILE__, __LINE__);  \
-    } while (0)
-
-inline cudaStream_t as_stream(void *s) { return reinterpret_cast<cudaStream_t>(s); }
 
 // ---------------------------------------------------------------- device buffer
 struct DevBuf

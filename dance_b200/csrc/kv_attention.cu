@@ -1,0 +1,788 @@
+// kv_attention.cu -- attention over the 8-bit key/value cache, over whole
+// sequences (dance_kv_attention) and over chosen blocks
+// (dance_kv_sparse_attention; include/dance_b200.h).
+//
+// Mathematics.  With codes k = kc - 128, v = vc - 128 (integers of 8 bits,
+// exact in half precision) and block scales sk, sv:
+//   s_j = scale * sk * (q . k_j),   o = sum_j p_j sv v_j / sum_j p_j,
+//   p_j = 2^(s_j log2 e - m), m the running maximum of the row.
+// Scales are constant in a block, so they stay out of the matrix products: sk
+// multiplies the logits, sv the weights.
+//
+// Roundings.  q enters as halves after an exact division by a power of two
+// per row (bfloat16 has fewer bits than half; what underflows is below 2^-38
+// of the row's largest channel).  The weights enter the second product as
+// halves of 2^14 p_j sv / (largest sv so far): 11 bits, and a weight counts
+// down to 2^-38 of the row's largest.  Products are summed in float, as are m,
+// the sum of the weights (taken before rounding) and the output.
+#include <cuda_runtime.h>
+
+#include "kv_common.cuh"
+
+namespace dance
+{
+namespace
+{
+
+constexpr int kWarps = 4;
+constexpr int kTile = 32;        // tokens of a warp's tile
+constexpr int kStages = 3;       // tiles of a warp in flight or in use
+constexpr int kEntries = 512;    // cache blocks looked up at once
+constexpr float kBoost = 14.0f;  // log2 of what a weight of 1 is as a half
+constexpr uint32_t kCounters = 1u << 16;
+constexpr int kMaxPos = 0x3FFFFFFF;
+
+struct AttnParams
+{
+    KvView c;
+    const uint16_t *q;
+    uint64_t q_row, q_head;
+    uint32_t rows, heads, G;
+    bool q_aligned;
+    float scale_log2;
+    const int32_t *blocks; // sparse: rows x hkv x select
+    uint32_t select;
+    uint32_t chunk;     // cache blocks of one split
+    uint32_t splits;    // most splits of a sequence
+    uint32_t row_tiles; // row tiles of a (sequence or row, head)
+    void *out;
+    float *lse;
+    uint32_t *counters;
+    float *part; // partial outputs, then partial log-sums
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Transpose of an 8 x 8 matrix of halves held one pair per lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two bytes of w (sel 0x4140: the low two, 0x4342: the high two) as the
+// halves c - 128.
+__device__ __forceinline__ uint32_t code_halves(uint32_t w, uint32_t sel)
+{
+    const uint32_t u = __byte_perm(w, 0x64646464u, sel);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+// Byte offset of 16-byte chunk ch of a tile's token in shared memory.  Keys
+// are read with four lanes along a token and eight tokens apart, values with
+// eight lanes along a token and four tokens apart by two; the offsets spread
+// either pattern over the banks.
+template <int D>
+__device__ __forceinline__ int key_off(int tok, int ch)
+{
+    return tok * D + (D == 128 ? (ch ^ ((tok & 1) << 2)) : ch) * 16;
+}
+template <int D>
+__device__ __forceinline__ int value_off(int tok, int ch)
+{
+    if constexpr (D == 128)
+        return tok * D + (ch ^ (tok & 6)) * 16;
+    else if constexpr (D == 64)
+        return (tok ^ ((tok >> 2) & 1)) * D + (ch ^ (tok & 2)) * 16;
+    else
+        return tok * D + ch * 16;
+}
+
+// Key words (4 codes) of lane t along a token: D / 16 words from t * D / 4.
+template <int D>
+__device__ __forceinline__ void load_key(const uint8_t *tile, int tok, int t, uint32_t (&w)[D / 16])
+{
+    if constexpr (D == 128)
+    {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4 *>(&w[4 * i]) =
+                *reinterpret_cast<const uint4 *>(tile + key_off<D>(tok, 2 * t + i));
+    }
+    else if constexpr (D == 96)
+    {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            *reinterpret_cast<uint2 *>(&w[2 * i]) = *reinterpret_cast<const uint2 *>(tile + tok * D + t * 24 + 8 * i);
+    }
+    else
+        *reinterpret_cast<uint4 *>(&w[0]) = *reinterpret_cast<const uint4 *>(tile + key_off<D>(tok, t));
+}
+
+// Value words of lane g along a token: D / 32 words from g * D / 8.
+template <int D>
+__device__ __forceinline__ void load_value(const uint8_t *tile, int tok, int g, uint32_t (&w)[D / 32])
+{
+    if constexpr (D == 128)
+        *reinterpret_cast<uint4 *>(&w[0]) = *reinterpret_cast<const uint4 *>(tile + value_off<D>(tok, g));
+    else if constexpr (D == 96)
+    {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            w[i] = *reinterpret_cast<const uint32_t *>(tile + tok * D + g * 12 + 4 * i);
+    }
+    else
+        *reinterpret_cast<uint2 *>(&w[0]) =
+            *reinterpret_cast<const uint2 *>(tile + value_off<D>(tok, g >> 1) + 8 * (g & 1));
+}
+
+template <int D>
+constexpr int ring_bytes()
+{
+    return kWarps * kStages * 2 * kTile * D;
+}
+template <int D>
+constexpr int rows_smem()
+{
+    return ring_bytes<D>() + kEntries * 16;
+}
+
+// Attention of at most 8 * NT rows that share a key/value head over one split
+// of their tokens.  Tokens lie on the 16-row side of the matrix instruction
+// and rows on its 8-column side, for both products (S^T = K Q^T, O^T = V^T
+// P^T): one row per query head of a single token fills 8 columns where the
+// other way round it would leave half of 16 rows empty.
+//
+// The codes go from shared memory straight into the operand registers: the
+// order of channels in a product over channels is free, so a lane takes D / 4
+// adjacent key bytes (the rows of q are laid out alike), and so is the order
+// of the output's channels, so a lane takes D / 8 adjacent value bytes of its
+// tokens.  Every warp streams its own tiles of 32 tokens through its own ring
+// (no barrier between warps) and keeps its own maximum and sums; the warps,
+// and then the splits, are joined at the end, the splits by the block that
+// finishes last, in their order.
+template <int D, int NT, bool SPARSE, bool BF16>
+__global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
+{
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int kRows = 8 * NT, kSteps = D / 16, kV = D / 8;
+    int *s_blk = reinterpret_cast<int *>(smem + ring_bytes<D>());
+    int *s_pos = s_blk + kEntries;
+    float *s_kf = reinterpret_cast<float *>(s_pos + kEntries);
+    float *s_vs = s_kf + kEntries;
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t b = blockIdx.y;
+    const uint32_t rt = blockIdx.x % p.row_tiles;
+    uint32_t xq = blockIdx.x / p.row_tiles;
+    const uint32_t h = xq % p.c.hkv;
+    xq /= p.c.hkv;
+    const uint32_t split = xq % p.splits;
+    const int tok = SPARSE ? (int)(xq / p.splits) : 0; // sparse: the row of the sequence
+    const KvSeq s = kv_seq(p.c, b, p.rows);
+    const int shift = (int)p.c.shift, bs = 1 << shift, G = (int)p.G;
+    const int r0 = (int)rt * kRows;
+    const int nrows = SPARSE ? (tok < s.rows ? G : 0) : s.rows * G;
+    if (r0 >= nrows)
+        return;
+    const int r1 = min(r0 + kRows, nrows);
+    const int tok_lo = SPARSE ? tok : r0 / G, tok_hi = SPARSE ? tok : (r1 - 1) / G;
+    const int seen_lo = min(s.first + tok_lo + 1, s.len), seen_hi = min(s.first + tok_hi + 1, s.len);
+    const int nent = SPARSE ? (int)p.select : (max(seen_hi, 0) + bs - 1) >> shift;
+    const int nsplits = max(1, (nent + (int)p.chunk - 1) / (int)p.chunk);
+    if ((int)split >= nsplits)
+        return;
+    const int e0 = (int)split * (int)p.chunk, e1 = min(e0 + (int)p.chunk, nent);
+
+    // ---- q as the second operand: lane (g, t) holds channels t * D/4 ... of rows 8 j + g
+    uint32_t qf[NT][2 * kSteps];
+    float rf[NT][2];   // logit factor of columns 2t, 2t + 1
+    int limit[NT][2];  // tokens that they see
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+    {
+        const int r = r0 + 8 * j + g;
+        float x[D / 4];
+        const bool live = r < r1;
+        const int i = SPARSE ? tok : r / G, hd = (int)h * G + (SPARSE ? r : r % G);
+        const uint16_t *src = p.q + (uint64_t)(s.row0 + (live ? i : 0)) * p.q_row + (uint64_t)(live ? hd : 0) * p.q_head +
+                              t * (D / 4);
+        if (p.q_aligned)
+        {
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e)
+            {
+                const uint4 w = __ldg(reinterpret_cast<const uint4 *>(src) + e);
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    x[8 * e + k] = kv_float<BF16>((uint16_t)(u[k >> 1] >> (16 * (k & 1))));
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int e = 0; e < D / 4; ++e)
+                x[e] = kv_float<BF16>(src[e]);
+        }
+        float amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < D / 4; ++e)
+            amax = fmaxf(amax, fabsf(x[e]));
+        amax = fmaxf(amax, __shfl_xor_sync(kKvFull, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(kKvFull, amax, 2));
+        // 2^(13 - exponent): the largest channel lands in [2^13, 2^14)
+        const int ex = (int)(__float_as_uint(amax) >> 23);
+        const int up = (ex == 255 || amax == 0.0f) ? 0 : min(126, 127 + 13 - ex);
+        const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
+        const float back = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+        for (int e = 0; e < 2 * kSteps; ++e)
+            qf[j][e] = live ? kv_pack<false>(x[2 * e] * mul, x[2 * e + 1] * mul) : 0u;
+        const float f = live ? back * p.scale_log2 : 0.0f;
+        rf[j][0] = __shfl_sync(kKvFull, f, (2 * t) << 2);
+        rf[j][1] = __shfl_sync(kKvFull, f, (2 * t + 1) << 2);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+        {
+            const int rr = min(r0 + 8 * j + 2 * t + k, r1 - 1);
+            limit[j][k] = min(s.first + (SPARSE ? tok : rr / G) + 1, s.len);
+        }
+    }
+
+    float o[kSteps][NT][4];
+    float m[NT][2], l[NT][2], vref = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+    {
+        m[j][0] = m[j][1] = kKvNegInf;
+        l[j][0] = l[j][1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+            o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
+    }
+    uint8_t *ring = smem + warp * (kStages * 2 * kTile * D);
+
+    for (int seg = e0; seg < e1; seg += kEntries)
+    {
+        const int ne = min(kEntries, e1 - seg);
+        const int ntiles = (ne * bs + kTile - 1) / kTile;
+        const int padded = min(kEntries, max(ne, (ntiles * kTile) >> shift)); // block_tokens 16: an even count
+        if (seg > e0)
+            __syncthreads();
+        for (int e = threadIdx.x; e < padded; e += kWarps * 32)
+        {
+            int page = -1;
+            if (e < ne)
+                page = SPARSE ? __ldg(p.blocks + ((uint64_t)(s.row0 + tok) * p.c.hkv + h) * p.select + seg + e)
+                              : seg + e;
+            int blk = -1;
+            if (page >= 0 && page < (kMaxPos >> shift) && (page << shift) < seen_hi)
+                blk = kv_block(p.c, b, page);
+            s_blk[e] = blk;
+            s_pos[e] = blk >= 0 ? page << shift : kMaxPos;
+            const uint64_t si = (uint64_t)max(blk, 0) * p.c.hkv + h;
+            s_kf[e] = blk >= 0 ? __ldg(p.c.ks + si) : 0.0f;
+            s_vs[e] = blk >= 0 ? __ldg(p.c.vs + si) : 0.0f;
+        }
+        __syncthreads();
+
+        auto issue = [&](int tile, int stage) {
+            if (tile < ntiles)
+            {
+                const int vt = tile * kTile;
+                uint8_t *kd = ring + stage * (2 * kTile * D), *vd = kd + kTile * D;
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                {
+                    const int v0 = vt + 16 * half, e = v0 >> shift;
+                    const int blk = s_blk[e];
+                    if (blk < 0)
+                        continue;
+                    const uint64_t off = (uint64_t)(((h << shift) + (uint32_t)(v0 & (bs - 1))) * D);
+                    const uint8_t *ksrc = p.c.k + (uint64_t)blk * p.c.kbs + off;
+                    const uint8_t *vsrc = p.c.v + (uint64_t)blk * p.c.vbs + off;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i)
+                    {
+                        const int cidx = lane + 32 * i, tk = 16 * half + cidx / (D / 16), ch = cidx % (D / 16);
+                        cp_async16(smem_addr(kd + key_off<D>(tk, ch)), ksrc + cidx * 16);
+                        cp_async16(smem_addr(vd + value_off<D>(tk, ch)), vsrc + cidx * 16);
+                    }
+                }
+            }
+            cp_async_commit();
+        };
+
+        for (int st = 0; st < kStages - 1; ++st)
+            issue(warp + kWarps * st, st);
+        int stage = 0;
+        for (int tile = warp; tile < ntiles; tile += kWarps)
+        {
+            int next = stage + kStages - 1;
+            next = next >= kStages ? next - kStages : next;
+            issue(tile + kWarps * (kStages - 1), next);
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            const uint8_t *kt = ring + stage * (2 * kTile * D), *vtile = kt + kTile * D;
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+            const int ea = (tile * kTile) >> shift, eb = (tile * kTile + 16) >> shift;
+            const int in_page = (tile * kTile) & (bs - 1);
+            const int pos[2] = {s_pos[ea] + in_page, s_pos[eb] + (eb == ea ? in_page + 16 : 0)};
+            if (pos[0] >= seen_hi && pos[1] >= seen_hi)
+            {
+                __syncwarp();
+                continue;
+            }
+            const float kf[2] = {s_kf[ea], s_kf[eb]}, vs[2] = {s_vs[ea], s_vs[eb]};
+
+            // ---- logits
+            float sc[2][NT][4];
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+            {
+                uint32_t ka[D / 16], kb[D / 16];
+                load_key<D>(kt, 16 * mt + g, t, ka);
+                load_key<D>(kt, 16 * mt + g + 8, t, kb);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    sc[mt][j][0] = sc[mt][j][1] = sc[mt][j][2] = sc[mt][j][3] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+                {
+                    const uint32_t a0 = code_halves(ka[i], 0x4140), a2 = code_halves(ka[i], 0x4342);
+                    const uint32_t a1 = code_halves(kb[i], 0x4140), a3 = code_halves(kb[i], 0x4342);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        mma_f16(sc[mt][j], a0, a1, a2, a3, qf[j][2 * i], qf[j][2 * i + 1]);
+                }
+            }
+            const bool whole = pos[0] + 16 <= seen_lo && pos[1] + 16 <= seen_lo;
+            bool up = false;
+            float mn[NT][2];
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+            {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                {
+                    float top = m[j][k];
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt)
+                    {
+                        const float f = kf[mt] * rf[j][k];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                        {
+                            float x = sc[mt][j][2 * u + k] * f;
+                            if (!whole && pos[mt] + g + 8 * u >= limit[j][k])
+                                x = kKvNegInf;
+                            sc[mt][j][2 * u + k] = x;
+                            top = fmaxf(top, x);
+                        }
+                    }
+                    top = fmaxf(top, __shfl_xor_sync(kKvFull, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(kKvFull, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(kKvFull, top, 16));
+                    mn[j][k] = top;
+                    up |= top > m[j][k];
+                }
+            }
+            const float vmax = fmaxf(vs[0], vs[1]);
+            if (__any_sync(kKvFull, up) || vmax > vref)
+            {
+                const float vn = fmaxf(vref, vmax);
+                const float vdown = vn > 0.0f ? __fdividef(vref, vn) : 1.0f;
+                vref = vn;
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                {
+                    float down[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                    {
+                        down[k] = mn[j][k] == kKvNegInf ? 1.0f : exp2_fast(m[j][k] - mn[j][k]);
+                        l[j][k] *= down[k];
+                        m[j][k] = mn[j][k];
+                        down[k] *= vdown;
+                    }
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i)
+                    {
+                        o[i][j][0] *= down[0];
+                        o[i][j][1] *= down[1];
+                        o[i][j][2] *= down[0];
+                        o[i][j][3] *= down[1];
+                    }
+                }
+            }
+
+            // ---- weights and their product with the values
+            const float vinv = vref > 0.0f ? __fdividef(1.0f, vref) : 0.0f;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+            {
+                const float vf = vs[mt] * vinv;
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                {
+                    const float m0 = m[j][0] == kKvNegInf ? 0.0f : m[j][0] - kBoost;
+                    const float m1 = m[j][1] == kKvNegInf ? 0.0f : m[j][1] - kBoost;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                    {
+                        const float p0 = exp2_fast(sc[mt][j][2 * u] - m0), p1 = exp2_fast(sc[mt][j][2 * u + 1] - m1);
+                        l[j][0] += p0;
+                        l[j][1] += p1;
+                        pb[j][u] = transpose8(kv_pack<false>(p0 * vf, p1 * vf));
+                    }
+                }
+                uint32_t v0[D / 32], v1[D / 32], v8[D / 32], v9[D / 32];
+                load_value<D>(vtile, 16 * mt + 2 * t, g, v0);
+                load_value<D>(vtile, 16 * mt + 2 * t + 1, g, v1);
+                load_value<D>(vtile, 16 * mt + 2 * t + 8, g, v8);
+                load_value<D>(vtile, 16 * mt + 2 * t + 9, g, v9);
+#pragma unroll
+                for (int w = 0; w < D / 32; ++w)
+                {
+                    // bytes of two tokens side by side: the pair of a channel is one operand register
+                    const uint32_t a_lo = __byte_perm(v0[w], v1[w], 0x5140), a_hi = __byte_perm(v0[w], v1[w], 0x7362);
+                    const uint32_t b_lo = __byte_perm(v8[w], v9[w], 0x5140), b_hi = __byte_perm(v8[w], v9[w], 0x7362);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                    {
+                        const uint32_t aw = u ? a_hi : a_lo, bw = u ? b_hi : b_lo;
+                        const uint32_t a0 = code_halves(aw, 0x4140), a1 = code_halves(aw, 0x4342);
+                        const uint32_t a2 = code_halves(bw, 0x4140), a3 = code_halves(bw, 0x4342);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+                            mma_f16(o[2 * w + u][j], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        cp_async_wait<0>();
+    }
+
+    // ---- the warps are joined: maxima and sums through shared memory, then the outputs
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+        {
+            l[j][k] += __shfl_xor_sync(kKvFull, l[j][k], 4);
+            l[j][k] += __shfl_xor_sync(kKvFull, l[j][k], 8);
+            l[j][k] += __shfl_xor_sync(kKvFull, l[j][k], 16);
+        }
+    __syncthreads();
+    float *s_o = reinterpret_cast<float *>(smem);         // kWarps x kRows x D
+    float *s_m = s_o + kWarps * kRows * D;                // kWarps x kRows
+    float *s_l = s_m + kWarps * kRows;                    // kWarps x kRows
+    float *s_all = s_l + kWarps * kRows;                  // 1 / sum of the rows
+    static_assert(4 * (kWarps * kRows * D + 2 * kWarps * kRows + kRows) <= ring_bytes<D>(), "join area");
+    if (g == 0)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+            {
+                s_m[warp * kRows + 8 * j + 2 * t + k] = m[j][k];
+                s_l[warp * kRows + 8 * j + 2 * t + k] = l[j][k];
+            }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+        {
+            const int r = 8 * j + 2 * t + k;
+            float top = kKvNegInf;
+            for (int w = 0; w < kWarps; ++w)
+                top = fmaxf(top, s_m[w * kRows + r]);
+            const float f = (m[j][k] == kKvNegInf ? 0.0f : exp2_fast(m[j][k] - top)) * vref;
+            float *dst = s_o + (warp * kRows + r) * D + g * kV;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                *reinterpret_cast<float2 *>(dst + 2 * i) = make_float2(o[i][j][k] * f, o[i][j][2 + k] * f);
+        }
+    __syncthreads();
+    const int item = (int)((SPARSE ? ((b * p.c.max_rows + (uint32_t)tok) * p.c.hkv + h) : (b * p.c.hkv + h)) *
+                               p.row_tiles + rt);
+    // partial results of the item (not touched where one split covers it)
+    float *part = p.part + (uint64_t)item * p.splits * kRows * (D + 1);
+    float *part_lse = part + (uint64_t)p.splits * kRows * D;
+    if (threadIdx.x < kRows)
+    {
+        const int r = threadIdx.x;
+        float top = kKvNegInf, sum = 0.0f;
+        for (int w = 0; w < kWarps; ++w)
+            top = fmaxf(top, s_m[w * kRows + r]);
+        // a maximum of -inf: no token (sum 0), or logits that are not numbers (sum NaN), which have to show
+        for (int w = 0; w < kWarps; ++w)
+            sum += s_m[w * kRows + r] == kKvNegInf ? s_l[w * kRows + r]
+                                                   : exp2_fast(s_m[w * kRows + r] - top) * s_l[w * kRows + r];
+        const float lse2 = sum == 0.0f ? kKvNegInf : top + log2f(sum) - kBoost;
+        s_all[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (nsplits > 1)
+            part_lse[split * kRows + r] = lse2;
+        else if (p.lse && r0 + r < r1)
+        {
+            const int i = SPARSE ? tok : (r0 + r) / G, hd = (int)h * G + (SPARSE ? r0 + r : (r0 + r) % G);
+            p.lse[(uint64_t)(s.row0 + i) * p.heads + hd] = lse2 * 0.69314718056f;
+        }
+    }
+    __syncthreads();
+    uint16_t *out = reinterpret_cast<uint16_t *>(p.out);
+    for (int e = threadIdx.x; e < kRows * D / 4; e += kWarps * 32)
+    {
+        const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+        if (r0 + r >= r1)
+            break;
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int w = 0; w < kWarps; ++w)
+        {
+            const float4 z = *reinterpret_cast<const float4 *>(s_o + (w * kRows + r) * D + d);
+            y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+        }
+        const float f = s_all[r];
+        y.x *= f, y.y *= f, y.z *= f, y.w *= f;
+        if (nsplits > 1)
+            *reinterpret_cast<float4 *>(part + ((uint64_t)split * kRows + r) * D + d) = y;
+        else
+        {
+            const int i = SPARSE ? tok : (r0 + r) / G, hd = (int)h * G + (SPARSE ? r0 + r : (r0 + r) % G);
+            *reinterpret_cast<uint2 *>(out + ((uint64_t)(s.row0 + i) * p.heads + hd) * D + d) =
+                make_uint2(kv_pack<BF16>(y.x, y.y), kv_pack<BF16>(y.z, y.w));
+        }
+    }
+    if (nsplits == 1)
+        return;
+
+    // ---- the splits are joined by the block that comes last, in their order
+    __shared__ bool s_last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0)
+        s_last = atomicAdd(p.counters + item, 1u) == (uint32_t)nsplits - 1u;
+    __syncthreads();
+    if (!s_last)
+        return;
+    __threadfence();
+    float *s_w = reinterpret_cast<float *>(smem); // kRows: 1 / sum, kRows: maximum
+    if (threadIdx.x < kRows)
+    {
+        const int r = threadIdx.x;
+        float top = kKvNegInf, sum = 0.0f;
+        for (int i = 0; i < nsplits; ++i)
+            top = fmaxf(top, __ldcg(part_lse + i * kRows + r));
+        const float base = top == kKvNegInf ? 0.0f : top;
+        for (int i = 0; i < nsplits; ++i)
+            sum += exp2_fast(__ldcg(part_lse + i * kRows + r) - base);
+        s_w[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        s_w[kRows + r] = base;
+        if (p.lse && r0 + r < r1)
+        {
+            const int i = SPARSE ? tok : (r0 + r) / G, hd = (int)h * G + (SPARSE ? r0 + r : (r0 + r) % G);
+            p.lse[(uint64_t)(s.row0 + i) * p.heads + hd] = (sum == 0.0f ? kKvNegInf : base + log2f(sum)) * 0.69314718056f;
+        }
+    }
+    if (threadIdx.x == 0)
+        p.counters[item] = 0u;
+    __syncthreads();
+    for (int e = threadIdx.x; e < kRows * D / 4; e += kWarps * 32)
+    {
+        const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+        if (r0 + r >= r1)
+            break;
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i = 0; i < nsplits; ++i)
+        {
+            const float w = exp2_fast(__ldcg(part_lse + i * kRows + r) - s_w[kRows + r]);
+            const float4 z = __ldcg(reinterpret_cast<const float4 *>(part + ((uint64_t)i * kRows + r) * D + d));
+            y.x += w * z.x, y.y += w * z.y, y.z += w * z.z, y.w += w * z.w;
+        }
+        const float f = s_w[r];
+        const int i = SPARSE ? tok : (r0 + r) / G, hd = (int)h * G + (SPARSE ? r0 + r : (r0 + r) % G);
+        *reinterpret_cast<uint2 *>(out + ((uint64_t)(s.row0 + i) * p.heads + hd) * D + d) =
+            make_uint2(kv_pack<BF16>(y.x * f, y.y * f), kv_pack<BF16>(y.z * f, y.w * f));
+    }
+}
+
+// How a call is cut: rows of a tile, splits, workspace.
+struct AttnPlan
+{
+    uint32_t nt, row_tiles, chunk, splits;
+    uint64_t items, blocks_x, bytes;
+};
+
+constexpr uint32_t kSlots = 2 * 148; // blocks of rows_kernel that the GPU holds at once
+
+AttnPlan plan_rows(const DanceKvCache &c, const DanceKvBatch &b, uint32_t heads, uint32_t select)
+{
+    AttnPlan a;
+    const uint32_t G = heads / c.kv_heads;
+    const uint64_t rows = select ? G : (uint64_t)b.max_rows * G;
+    a.nt = rows <= 8 ? 1u : 2u;
+    a.row_tiles = (uint32_t)((rows + 8 * a.nt - 1) / (8 * a.nt));
+    const uint64_t per_b = (uint64_t)c.kv_heads * a.row_tiles * (select ? b.max_rows : 1u);
+    a.items = per_b * b.batch;
+    const uint64_t len = b.max_len < (uint64_t)b.table_width * c.block_tokens ? b.max_len
+                                                                             : (uint64_t)b.table_width * c.block_tokens;
+    const uint32_t ent = select ? select : (uint32_t)((len + c.block_tokens - 1) / c.block_tokens);
+    // splits: about four waves of blocks, none under 256 tokens
+    uint64_t want = (4 * kSlots + a.items - 1) / (a.items ? a.items : 1);
+    const uint64_t most = ((uint64_t)ent * c.block_tokens + 255) / 256;
+    want = want > most ? most : want;
+    if (want < 1 || a.items > kCounters)
+        want = 1;
+    a.chunk = (uint32_t)((ent + want - 1) / want);
+    if (c.block_tokens == 16)
+        a.chunk += a.chunk & 1u;
+    a.chunk = a.chunk ? a.chunk : 1;
+    a.splits = (ent + a.chunk - 1) / a.chunk;
+    a.splits = a.splits ? a.splits : 1;
+    a.blocks_x = per_b * a.splits;
+    a.bytes = kCounters * 4ull + (a.splits > 1 ? a.items * a.splits * 8 * a.nt * (c.head_dim + 1) * 4ull : 0ull);
+    return a;
+}
+
+template <int D, int NT, bool SPARSE, bool BF16>
+int launch_rows(const AttnParams &p, dim3 grid, cudaStream_t st)
+{
+    static const cudaError_t attr = cudaFuncSetAttribute(rows_kernel<D, NT, SPARSE, BF16>,
+                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem<D>());
+    DANCE_CUDA(attr);
+    rows_kernel<D, NT, SPARSE, BF16><<<grid, kWarps * 32, rows_smem<D>(), st>>>(p);
+    DANCE_LAUNCHED();
+    return 0;
+}
+
+template <int D>
+int launch_rows_d(const AttnParams &p, uint32_t nt, bool bf16, dim3 grid, cudaStream_t st)
+{
+    const bool sparse = p.blocks != nullptr;
+    switch ((nt - 1) * 4 + (sparse ? 2 : 0) + (bf16 ? 1 : 0))
+    {
+    case 0:
+        return launch_rows<D, 1, false, false>(p, grid, st);
+    case 1:
+        return launch_rows<D, 1, false, true>(p, grid, st);
+    case 2:
+        return launch_rows<D, 1, true, false>(p, grid, st);
+    case 3:
+        return launch_rows<D, 1, true, true>(p, grid, st);
+    case 4:
+        return launch_rows<D, 2, false, false>(p, grid, st);
+    case 5:
+        return launch_rows<D, 2, false, true>(p, grid, st);
+    case 6:
+        return launch_rows<D, 2, true, false>(p, grid, st);
+    default:
+        return launch_rows<D, 2, true, true>(p, grid, st);
+    }
+}
+
+int attend(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *q, uint32_t num_heads,
+           const int32_t *d_blocks, uint32_t select, float scale, void *d_out, float *d_lse, void *d_workspace,
+           uint64_t workspace_bytes, void *stream)
+{
+    if (int rc = kv_check(cache, batch))
+        return rc;
+    if (int rc = kv_check_rows(q, cache->head_dim, num_heads, "q"))
+        return rc;
+    if (num_heads == 0 || num_heads % cache->kv_heads || num_heads > 65536)
+        return fail(-1, "num_heads %u must be a multiple of kv_heads %u", num_heads, cache->kv_heads);
+    if (q->rows == 0 || batch->max_rows == 0)
+        return 0;
+    if (!d_out || (uintptr_t)d_out % 16 || (uintptr_t)d_lse % 4)
+        return fail(-1, "null or misaligned output");
+    const AttnPlan a = plan_rows(*cache, *batch, num_heads, select);
+    if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < a.bytes)
+        return fail(-1, "workspace of %llu bytes: %llu are needed", (unsigned long long)workspace_bytes,
+                    (unsigned long long)a.bytes);
+    if (a.blocks_x > 0x7FFFFFFFull)
+        return fail(-1, "call too large: %llu thread blocks per sequence", (unsigned long long)a.blocks_x);
+    AttnParams p;
+    p.c = kv_view(*cache, *batch);
+    p.q = reinterpret_cast<const uint16_t *>(q->d_data);
+    p.q_row = q->row_stride;
+    p.q_head = q->head_stride;
+    p.q_aligned = kv_aligned(*q);
+    p.rows = q->rows;
+    p.heads = num_heads;
+    p.G = num_heads / cache->kv_heads;
+    p.scale_log2 = scale * 1.44269504089f;
+    p.blocks = d_blocks;
+    p.select = select;
+    p.chunk = a.chunk;
+    p.splits = a.splits;
+    p.row_tiles = a.row_tiles;
+    p.out = d_out;
+    p.lse = d_lse;
+    p.counters = reinterpret_cast<uint32_t *>(d_workspace);
+    p.part = reinterpret_cast<float *>(p.counters + kCounters);
+    const dim3 grid((unsigned)a.blocks_x, batch->batch);
+    const bool bf16 = q->dtype == DANCE_BF16;
+    switch (cache->head_dim)
+    {
+    case 64:
+        return launch_rows_d<64>(p, a.nt, bf16, grid, as_stream(stream));
+    case 96:
+        return launch_rows_d<96>(p, a.nt, bf16, grid, as_stream(stream));
+    default:
+        return launch_rows_d<128>(p, a.nt, bf16, grid, as_stream(stream));
+    }
+}
+
+} // namespace
+
+uint64_t kv_counter_bytes() { return kCounters * 4ull; }
+uint64_t kv_attention_bytes(const DanceKvCache &c, const DanceKvBatch &b, uint32_t heads, uint32_t select)
+{
+    return plan_rows(c, b, heads, select).bytes;
+}
+
+} // namespace dance
+
+using namespace dance;
+
+extern "C" int dance_kv_attention(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *q,
+                                  uint32_t num_heads, float scale, void *d_out, float *d_lse, void *d_workspace,
+                                  uint64_t workspace_bytes, void *stream)
+{
+    return attend(cache, batch, q, num_heads, nullptr, 0, scale, d_out, d_lse, d_workspace, workspace_bytes, stream);
+}
+
+extern "C" int dance_kv_sparse_attention(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *q,
+                                         uint32_t num_heads, const int32_t *d_blocks, uint32_t select, float scale,
+                                         void *d_out, float *d_lse, void *d_workspace, uint64_t workspace_bytes,
+                                         void *stream)
+{
+    if (!d_blocks || (uintptr_t)d_blocks % 4)
+        return fail(-1, "null or misaligned block selection");
+    if (select == 0 || select > 4096)
+        return fail(-1, "select %u: 1 to 4096 are supported", select);
+    return attend(cache, batch, q, num_heads, d_blocks, select, scale, d_out, d_lse, d_workspace, workspace_bytes,
+                  stream);
+}

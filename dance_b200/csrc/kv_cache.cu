@@ -1,0 +1,347 @@
+// kv_cache.cu -- the write into and the read out of the 8-bit key/value cache
+// (dance_kv_append, dance_kv_read in include/dance_b200.h).
+//
+// append.  One thread block per (touched cache block, head, keys or values).
+// Its new rows are read once into registers; their largest finite magnitude
+// and the scale so far give the new scale.  Only where that grew are the
+// block's earlier codes read, rounded again and written back.  The earlier
+// tokens enter the bounds through the bounds themselves (rounding is monotone,
+// so the rounded bounds are the bounds of the rounded codes), so that a decode
+// step moves one token and 2 * head_dim bytes of bounds, not a block.
+// Threads are laid out as 16 token groups x head_dim / 8 channel groups: a
+// thread keeps its 8 channels through all its tokens, so the bounds are byte
+// minima and maxima in registers and one reduction over 16 groups.
+//
+// Both kernels move each byte once and are bound by memory on prompts and by
+// latency on single tokens.
+#include "kv_common.cuh"
+
+namespace dance
+{
+namespace
+{
+
+constexpr int kTokenGroups = 16;
+
+struct AppendParams
+{
+    KvView c;
+    const uint16_t *x[2]; // new keys, new values
+    uint64_t row_stride[2], head_stride[2];
+    uint32_t rows;
+    bool aligned[2];
+};
+
+// The largest of a non-negative value over the thread block.
+__device__ __forceinline__ float block_max(float x, float *s)
+{
+    for (int o = 16; o; o >>= 1)
+        x = fmaxf(x, __shfl_xor_sync(kKvFull, x, o));
+    if ((threadIdx.x & 31) == 0)
+        s[threadIdx.x >> 5] = x;
+    __syncthreads();
+    float m = 0.0f;
+    for (int i = 0; i < (int)blockDim.x / 32; ++i)
+        m = fmaxf(m, s[i]);
+    return m;
+}
+
+// Four codes rounded again to a scale that is 1 / shrink times as large.
+__device__ __forceinline__ uint32_t shrink_codes(uint32_t w, float shrink)
+{
+    uint32_t r = 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+    {
+        const float y = __fmul_rn((float)((int)((w >> (8 * e)) & 255u) - 128), shrink);
+        r |= ((uint32_t)(__float2int_rn(y) + 128) & 255u) << (8 * e);
+    }
+    return r;
+}
+
+// IT = block_tokens / 16 tokens per thread.
+template <int D, int IT, bool BF16>
+__global__ void __launch_bounds__(D / 8 * kTokenGroups) append_kernel(AppendParams p)
+{
+    constexpr int kD8 = D / 8, kBs = IT * kTokenGroups;
+    __shared__ float red[8];
+    __shared__ uint2 lo_s[kTokenGroups][kD8], hi_s[kTokenGroups][kD8];
+    const uint32_t b = blockIdx.z, h = blockIdx.y >> 1, kind = blockIdx.y & 1u;
+    const KvSeq s = kv_seq(p.c, b, p.rows);
+    const int start = max(s.first, 0), end = s.first + s.rows;
+    const int page = start / kBs + (int)blockIdx.x;
+    const int base = page * kBs;
+    const int lo = max(start, base), hi = min(end, base + kBs);
+    if (lo >= hi)
+        return;
+    const int blk = kv_block(p.c, b, page);
+    if (blk < 0)
+        return;
+    const int n_old = lo - base;
+    const int d8 = threadIdx.x % kD8, tg = threadIdx.x / kD8;
+    const uint64_t si = (uint64_t)blk * p.c.hkv + h;
+    uint8_t *codes = (kind ? p.c.v + (uint64_t)blk * p.c.vbs : p.c.k + (uint64_t)blk * p.c.kbs) +
+                     (uint64_t)h * (kBs * D) + d8 * 8;
+    float *scales = kind ? p.c.vs : p.c.ks;
+    const uint16_t *x0 = p.x[kind] + (uint64_t)h * p.head_stride[kind] + d8 * 8;
+    const float old = n_old ? scales[si] : 0.0f;
+
+    uint4 x[IT];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+    {
+        const int pos = base + tg + kTokenGroups * i;
+        x[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (pos >= lo && pos < hi)
+        {
+            const uint16_t *src = x0 + (uint64_t)(s.row0 + pos - s.first) * p.row_stride[kind];
+            if (p.aligned[kind])
+                x[i] = __ldg(reinterpret_cast<const uint4 *>(src));
+            else
+            {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
+                x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+    {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+        {
+            amax = fmaxf(amax, kv_finite_abs(kv_float<BF16>((uint16_t)w[e])));
+            amax = fmaxf(amax, kv_finite_abs(kv_float<BF16>((uint16_t)(w[e] >> 16))));
+        }
+    }
+    amax = block_max(amax, red);
+    const float scale = fmaxf(old, kv_scale_of(amax));
+    const float inv = kv_inverse(scale);
+    // a scale that was never written (NaN) cannot be told from a grown one: the comparison treats it as grown
+    const bool grew = n_old > 0 && !(scale == old);
+    const float shrink = scale > 0.0f ? __fdiv_rn(old, scale) : 0.0f;
+
+    uint32_t lo4[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, hi4[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+    {
+        const int t = tg + kTokenGroups * i, pos = base + t;
+        if (pos >= lo && pos < hi)
+        {
+            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            uint32_t q[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+                q[2 * e] = (uint32_t)(kv_code(kv_float<BF16>((uint16_t)w[e]), inv) + 128);
+                q[2 * e + 1] = (uint32_t)(kv_code(kv_float<BF16>((uint16_t)(w[e] >> 16)), inv) + 128);
+            }
+            const uint32_t c2[2] = {q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24),
+                                    q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24)};
+            *reinterpret_cast<uint2 *>(codes + t * D) = make_uint2(c2[0], c2[1]);
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+            {
+                lo4[g] = __vminu4(lo4[g], c2[g]);
+                hi4[g] = __vmaxu4(hi4[g], c2[g]);
+            }
+        }
+        else if (grew && t < n_old)
+        {
+            const uint2 c = *reinterpret_cast<const uint2 *>(codes + t * D);
+            *reinterpret_cast<uint2 *>(codes + t * D) = make_uint2(shrink_codes(c.x, shrink), shrink_codes(c.y, shrink));
+        }
+    }
+    if (threadIdx.x == 0)
+        scales[si] = scale;
+    if (kind == 0)
+    {
+        lo_s[tg][d8] = make_uint2(lo4[0], lo4[1]);
+        hi_s[tg][d8] = make_uint2(hi4[0], hi4[1]);
+        __syncthreads();
+        if (threadIdx.x < 2 * kD8)
+        {
+            const bool high = threadIdx.x >= kD8;
+            const int d = high ? threadIdx.x - kD8 : threadIdx.x;
+            uint2 *out = reinterpret_cast<uint2 *>(p.c.bounds + (2 * si + (high ? 1 : 0)) * D) + d;
+            uint2 r = high ? make_uint2(0u, 0u) : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
+            if (n_old)
+            {
+                r = *out;
+                if (grew)
+                    r = make_uint2(shrink_codes(r.x, shrink), shrink_codes(r.y, shrink));
+            }
+            for (int g = 0; g < kTokenGroups; ++g)
+            {
+                const uint2 y = high ? hi_s[g][d] : lo_s[g][d];
+                r.x = high ? __vmaxu4(r.x, y.x) : __vminu4(r.x, y.x);
+                r.y = high ? __vmaxu4(r.y, y.y) : __vminu4(r.y, y.y);
+            }
+            *out = r;
+        }
+    }
+}
+
+template <int D>
+int launch_append(const AppendParams &p, dim3 grid, bool bf16, cudaStream_t st)
+{
+    const dim3 block(D / 8 * kTokenGroups);
+    switch (((1u << p.c.shift) / kTokenGroups) * 2 + (bf16 ? 1 : 0))
+    {
+#define DANCE_APPEND_CASE(it)                                                                                    \
+    case 2 * it:                                                                                                 \
+        append_kernel<D, it, false><<<grid, block, 0, st>>>(p);                                                  \
+        break;                                                                                                   \
+    case 2 * it + 1:                                                                                             \
+        append_kernel<D, it, true><<<grid, block, 0, st>>>(p);                                                   \
+        break;
+        DANCE_APPEND_CASE(1)
+        DANCE_APPEND_CASE(2)
+        DANCE_APPEND_CASE(4)
+        DANCE_APPEND_CASE(8)
+#undef DANCE_APPEND_CASE
+    default:
+        return fail(-1, "block_tokens %u", 1u << p.c.shift);
+    }
+    DANCE_LAUNCHED();
+    return 0;
+}
+
+// One thread per 8 channels of a (row, head): 8 code bytes in, 8 values out.
+template <int D, int DT>
+__global__ void __launch_bounds__(256) read_kernel(KvView c, uint32_t rows, void *ko, void *vo)
+{
+    constexpr uint32_t kD8 = D / 8;
+    const uint32_t b = blockIdx.y;
+    const KvSeq s = kv_seq(c, b, rows);
+    const uint64_t n = (uint64_t)s.rows * c.hkv * kD8;
+    const uint32_t mask = (1u << c.shift) - 1u;
+    for (uint64_t e = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (uint64_t)gridDim.x * blockDim.x)
+    {
+        const uint32_t d8 = (uint32_t)(e % kD8), rh = (uint32_t)(e / kD8), h = rh % c.hkv, i = rh / c.hkv;
+        const int pos = s.first + (int)i;
+        const int blk = pos >= 0 ? kv_block(c, b, pos >> c.shift) : -1;
+        const uint64_t si = (uint64_t)max(blk, 0) * c.hkv + h;
+        const uint64_t in = (((uint64_t)h << c.shift) + ((uint32_t)pos & mask)) * D + d8 * 8;
+        const uint64_t out = ((uint64_t)(s.row0 + i) * c.hkv + h) * D + d8 * 8;
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind)
+        {
+            void *dst = kind ? vo : ko;
+            if (!dst)
+                continue;
+            float y[8];
+            uint2 w = make_uint2(0x80808080u, 0x80808080u);
+            float scale = 0.0f;
+            if (blk >= 0)
+            {
+                w = __ldg(reinterpret_cast<const uint2 *>(
+                    (kind ? c.v + (uint64_t)blk * c.vbs : c.k + (uint64_t)blk * c.kbs) + in));
+                scale = __ldg((kind ? c.vs : c.ks) + si);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                y[k] = __fmul_rn((float)((int)(((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 255u) - 128), scale);
+            if constexpr (DT == DANCE_F32)
+            {
+                float4 *o = reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + out);
+                o[0] = make_float4(y[0], y[1], y[2], y[3]);
+                o[1] = make_float4(y[4], y[5], y[6], y[7]);
+            }
+            else
+            {
+                constexpr bool bf = DT == DANCE_BF16;
+                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(dst) + out) =
+                    make_uint4(kv_pack<bf>(y[0], y[1]), kv_pack<bf>(y[2], y[3]), kv_pack<bf>(y[4], y[5]),
+                               kv_pack<bf>(y[6], y[7]));
+            }
+        }
+    }
+}
+
+template <int D>
+int launch_read(const KvView &c, uint32_t rows, int dtype, void *ko, void *vo, cudaStream_t st)
+{
+    const uint64_t work = (uint64_t)c.max_rows * c.hkv * (D / 8);
+    const dim3 grid((unsigned)((work + 255) / 256 < 65536 ? (work + 255) / 256 : 65536), c.batch);
+    if (dtype == DANCE_F32)
+        read_kernel<D, DANCE_F32><<<grid, 256, 0, st>>>(c, rows, ko, vo);
+    else if (dtype == DANCE_F16)
+        read_kernel<D, DANCE_F16><<<grid, 256, 0, st>>>(c, rows, ko, vo);
+    else
+        read_kernel<D, DANCE_BF16><<<grid, 256, 0, st>>>(c, rows, ko, vo);
+    DANCE_LAUNCHED();
+    return 0;
+}
+
+} // namespace
+} // namespace dance
+
+using namespace dance;
+
+extern "C" int dance_kv_append(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *k,
+                               const DanceKvRows *v, void *stream)
+{
+    if (int rc = kv_check(cache, batch))
+        return rc;
+    if (int rc = kv_check_rows(k, cache->head_dim, cache->kv_heads, "k"))
+        return rc;
+    if (int rc = kv_check_rows(v, cache->head_dim, cache->kv_heads, "v"))
+        return rc;
+    if (k->rows != v->rows || k->dtype != v->dtype)
+        return fail(-1, "keys (%u rows, dtype %d) and values (%u rows, dtype %d) differ", k->rows, k->dtype, v->rows,
+                    v->dtype);
+    if (k->rows == 0 || batch->max_rows == 0)
+        return 0;
+    AppendParams p;
+    p.c = kv_view(*cache, *batch);
+    const DanceKvRows *r[2] = {k, v};
+    for (int i = 0; i < 2; ++i)
+    {
+        p.x[i] = reinterpret_cast<const uint16_t *>(r[i]->d_data);
+        p.row_stride[i] = r[i]->row_stride;
+        p.head_stride[i] = r[i]->head_stride;
+        p.aligned[i] = kv_aligned(*r[i]);
+    }
+    p.rows = k->rows;
+    const uint32_t bs = cache->block_tokens;
+    const dim3 grid((batch->max_rows + bs - 2) / bs + 1, 2 * cache->kv_heads, batch->batch);
+    const bool bf16 = k->dtype == DANCE_BF16;
+    switch (cache->head_dim)
+    {
+    case 64:
+        return launch_append<64>(p, grid, bf16, as_stream(stream));
+    case 96:
+        return launch_append<96>(p, grid, bf16, as_stream(stream));
+    default:
+        return launch_append<128>(p, grid, bf16, as_stream(stream));
+    }
+}
+
+extern "C" int dance_kv_read(const DanceKvCache *cache, const DanceKvBatch *batch, uint32_t rows, int dtype,
+                             void *d_k_out, void *d_v_out, void *stream)
+{
+    if (int rc = kv_check(cache, batch))
+        return rc;
+    if (dtype != DANCE_F16 && dtype != DANCE_BF16 && dtype != DANCE_F32)
+        return fail(-1, "output dtype %d: float16, bfloat16 and float32 are supported", dtype);
+    if (((uintptr_t)d_k_out | (uintptr_t)d_v_out) % 16)
+        return fail(-1, "outputs must be 16-byte aligned");
+    if (rows == 0 || batch->max_rows == 0 || (!d_k_out && !d_v_out))
+        return 0;
+    const KvView c = kv_view(*cache, *batch);
+    switch (cache->head_dim)
+    {
+    case 64:
+        return launch_read<64>(c, rows, dtype, d_k_out, d_v_out, as_stream(stream));
+    case 96:
+        return launch_read<96>(c, rows, dtype, d_k_out, d_v_out, as_stream(stream));
+    default:
+        return launch_read<128>(c, rows, dtype, d_k_out, d_v_out, as_stream(stream));
+    }
+}

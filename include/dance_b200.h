@@ -39,7 +39,8 @@ enum
 {
     DANCE_U8 = 0,  /* uint8, exact integer squared L2 */
     DANCE_F16 = 1, /* IEEE binary16 storage, half-precision diff/square as the reference */
-    DANCE_F32 = 2  /* float32 */
+    DANCE_F32 = 2, /* float32 */
+    DANCE_BF16 = 3 /* bfloat16: the key/value cache operators only */
 };
 
 /* Runtime form of the knobs in gpu_vamana_config.h (same names, lower case). */
@@ -436,6 +437,125 @@ DANCE_API int dance_partition_assign(int dtype, const void *d_data, uint64_t row
 DANCE_API int dance_partition_buckets(const uint32_t *d_assign, uint64_t num_points, uint32_t k_base,
                                       uint32_t num_shards, uint32_t *d_shard_offsets, uint32_t *d_shard_ids,
                                       void *stream);
+
+/* ---- key/value cache: append, read, attention, block selection ------------ */
+/* Long-context memory next to the index: a model's keys and values in 8 bits,
+ * and the attention over all of them or over the blocks that a cheap score (or
+ * a graph search over the keys) picked.  None of these calls synchronises or
+ * allocates; all may be captured in a CUDA graph.
+ *
+ * The cache is a pool of blocks of block_tokens (16, 32, 64 or 128) tokens.
+ * Block b, head h, token t, channel d of the keys is the byte
+ *   d_k[b * k_block_stride + (h * block_tokens + t) * head_dim + d],
+ * likewise the values; a code c stands for (c - 128) * scale with one float
+ * scale per block and head (d_k_scale, d_v_scale: num_blocks x kv_heads).
+ * d_k_bounds (num_blocks x kv_heads x 2 x head_dim) holds the smallest and
+ * the largest key code of every channel over the block's tokens.  head_dim
+ * is 64, 96 or 128; pointers and block strides are multiples of 16 bytes. */
+typedef struct DanceKvCache
+{
+    uint8_t *d_k;
+    uint8_t *d_v;
+    float *d_k_scale;
+    float *d_v_scale;
+    uint8_t *d_k_bounds;
+    uint64_t k_block_stride; /* bytes */
+    uint64_t v_block_stride; /* bytes */
+    uint32_t num_blocks;
+    uint32_t kv_heads;
+    uint32_t block_tokens;
+    uint32_t head_dim;
+} DanceKvCache;
+
+/* The sequences of one call, ragged.  Sequence b holds d_seq_lens[b] tokens,
+ * its new rows included; its rows of the call's tensors are
+ * d_row_offsets[b] .. d_row_offsets[b + 1], row i of r having position
+ * d_seq_lens[b] - r + i (a row of negative position sees nothing).  Its
+ * tokens lie in the blocks named by row b of d_block_table (batch x
+ * table_width); entries outside [0, num_blocks) hold no tokens: writes to
+ * them are dropped, reads see nothing there.  max_rows and max_len bound the
+ * rows and the length of every sequence (they size the launch; rows and
+ * tokens beyond them are not visited).  batch <= 65535. */
+typedef struct DanceKvBatch
+{
+    const int32_t *d_block_table;
+    const int32_t *d_seq_lens;
+    const int32_t *d_row_offsets;
+    uint32_t table_width;
+    uint32_t batch;
+    uint32_t max_rows;
+    uint32_t max_len;
+} DanceKvBatch;
+
+/* A dense tensor (rows x heads x head_dim) of DANCE_F16 or DANCE_BF16
+ * elements, channels contiguous; strides in elements. */
+typedef struct DanceKvRows
+{
+    const void *d_data;
+    uint64_t row_stride;
+    uint64_t head_stride;
+    uint32_t rows;
+    int dtype;
+} DanceKvRows;
+
+/* Writes the batch's new rows (k, v: rows x kv_heads) into the cache.  Per
+ * block and head, with x the new rows that fall into it:
+ *   scale' = max(scale if the block held tokens of the sequence before,
+ *                max |x| over finite x / 127), below 2^-126: 0;
+ *   codes held before: rint((c - 128) * (scale / scale')) + 128;
+ *   new codes: clamp(rint(x * (1 / scale')), -127, 127) + 128, NaN -> 128;
+ * in float, ties to even.  The bounds of a block that held tokens before are
+ * rounded as its codes are, and widened by the new codes; a block's first
+ * tokens set them.  (Rows may be written again at shorter lengths, as after a
+ * rejected draft: scales and bounds then stay as wide as they were.)  Two
+ * sequences of a call must not write the same block. */
+DANCE_API int dance_kv_append(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *k,
+                              const DanceKvRows *v, void *stream);
+/* The values that the cache holds for the batch's rows: (c - 128) * scale,
+ * rounded once to dtype (DANCE_F16, DANCE_BF16 or DANCE_F32), to d_k_out and
+ * d_v_out (rows x kv_heads x head_dim, contiguous, 16-byte aligned; either
+ * may be NULL).  Rows without tokens (negative position, no block) read 0. */
+DANCE_API int dance_kv_read(const DanceKvCache *cache, const DanceKvBatch *batch, uint32_t rows, int dtype,
+                            void *d_k_out, void *d_v_out, void *stream);
+/* Attention of the rows q (rows x num_heads; num_heads a multiple of
+ * kv_heads, query head h reading key/value head h / (num_heads / kv_heads))
+ * over their sequences' tokens up to their own position:
+ *   out = sum_j softmax_j(scale * q.k_j) v_j.
+ * d_out: rows x num_heads x head_dim of q's type, contiguous, 16-byte
+ * aligned; d_lse (optional): log sum_j exp(scale * q.k_j), rows x num_heads.
+ * A row that sees no token gets 0 and -inf.  d_workspace holds at least
+ * dance_kv_workspace_bytes(...) bytes, zeroed once before its first use; a
+ * workspace serves one call at a time. */
+DANCE_API int dance_kv_attention(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *q,
+                                 uint32_t num_heads, float scale, void *d_out, float *d_lse, void *d_workspace,
+                                 uint64_t workspace_bytes, void *stream);
+/* The blocks that each row reads: d_blocks (rows x kv_heads x select, -1
+ * filled) receives, ascending, the positions in the block table of the row's
+ * chosen blocks, among the blocks that hold positions up to its own: the
+ * first first_blocks and the last last_blocks of them, and the best of the
+ * rest up to select in all, by the score
+ *   max over the head's query heads of  s_q * B  times the block's key scale,
+ *   B = sum_d max(c_d * (low_d - 128), c_d * (high_d - 128)),
+ * c = clamp(rint(q * (1 / s_q)), -127, 127), s_q = max |q| over finite q / 127
+ * (below 2^-126: 0), low and high the block's bounds.  B is an integer; the
+ * two products are float, in this order.  Ties go to the lower block.
+ * select >= first_blocks + last_blocks, 1 <= select <= 4096. */
+DANCE_API int dance_kv_select_blocks(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *q,
+                                     uint32_t num_heads, uint32_t select, uint32_t first_blocks,
+                                     uint32_t last_blocks, int32_t *d_blocks, void *d_workspace,
+                                     uint64_t workspace_bytes, void *stream);
+/* Attention of each row over the tokens of the blocks in its row of d_blocks
+ * (rows x kv_heads x select, positions in the block table, negative or
+ * out-of-range entries skipped; a block named twice counts twice) up to its
+ * own position.  Otherwise as dance_kv_attention. */
+DANCE_API int dance_kv_sparse_attention(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *q,
+                                        uint32_t num_heads, const int32_t *d_blocks, uint32_t select, float scale,
+                                        void *d_out, float *d_lse, void *d_workspace, uint64_t workspace_bytes,
+                                        void *stream);
+/* Workspace bytes that the attention (select = 0), or the selection and the
+ * block-sparse attention (select > 0), of such a call can need. */
+DANCE_API uint64_t dance_kv_workspace_bytes(const DanceKvCache *cache, const DanceKvBatch *batch, uint32_t rows,
+                                            uint32_t num_heads, uint32_t select);
 
 #ifdef __cplusplus
 }
