@@ -10,9 +10,10 @@
 // of an integer sum does not show, so the choice is the same however it is
 // summed.
 //
-// scores_kernel writes the float scores of (row, head, block); choose_kernel
-// finds each (row, head)'s select-th largest key by a radix search over four
-// bytes and writes the chosen blocks in ascending order.
+// scores_kernel writes the float scores of (row, head, block) from integer
+// matrix instructions, choose_kernel finds each (row, head)'s threshold in
+// histograms of the order-preserving keys and writes the chosen blocks in
+// ascending order.
 #include "kv_common.cuh"
 
 namespace dance
@@ -21,8 +22,11 @@ namespace
 {
 
 constexpr int kScoreThreads = 128;
-constexpr int kScoreHeads = 8; // query heads scored together
+constexpr int kScoreBlocks = 128; // cache blocks of one pass of a thread block: 32 per warp
+constexpr int kScoreHeads = 8;    // query heads in shared memory at once
 constexpr int kChooseThreads = 256;
+constexpr int kBins = 2048;
+constexpr uint32_t kChooseKeys = 9728; // keys that the choice holds in shared memory
 
 struct SelectParams
 {
@@ -30,118 +34,217 @@ struct SelectParams
     const uint16_t *q;
     uint64_t q_row, q_head;
     uint32_t rows, heads, G;
-    uint32_t nblk; // scores of a (row, head)
+    uint32_t nblk;      // blocks that a row can see
+    uint32_t width;     // floats from one (row, head)'s scores to the next
+    uint32_t row_tiles; // of a sequence
+    uint32_t passes;    // runs of blocks of a thread block
+    uint32_t slots;     // query heads in shared memory at once
     uint32_t select, first, last;
     float *scores; // rows x hkv x nblk
     int32_t *out;
 };
 
-// One thread block per (row, head, 128 blocks), one thread per block.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kScoreThreads) scores_kernel(SelectParams p)
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1)
 {
-    __shared__ __align__(16) uint32_t c_s[kScoreHeads][D / 2]; // c+ of the channels, then c-
-    __shared__ float qs_s[kScoreHeads];
-    __shared__ int sum_s[kScoreHeads];
-    const uint32_t b = blockIdx.z, h = blockIdx.y % p.c.hkv;
-    const int i = (int)(blockIdx.y / p.c.hkv);
-    const KvSeq s = kv_seq(p.c, b, p.rows);
-    if (i >= s.rows)
-        return;
-    const int seen = min(s.first + i + 1, s.len);
-    const int nb = (max(seen, 0) + (1 << p.c.shift) - 1) >> p.c.shift;
-    const int j0 = (int)blockIdx.x * kScoreThreads;
-    if (j0 >= nb)
-        return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int j = j0 + (int)threadIdx.x;
-    const int blk = j < nb ? kv_block(p.c, b, j) : -1;
-    uint4 w[D / 8];
-    if (blk >= 0)
-    {
-        const uint4 *src = reinterpret_cast<const uint4 *>(p.c.bounds + ((uint64_t)blk * p.c.hkv + h) * 2 * D);
-#pragma unroll
-        for (int e = 0; e < D / 8; ++e)
-            w[e] = __ldg(src + e);
-    }
-    const float ks = blk >= 0 ? __ldg(p.c.ks + (uint64_t)blk * p.c.hkv + h) : 0.0f;
-    float best = kKvNegInf;
-    for (uint32_t g0 = 0; g0 < p.G; g0 += kScoreHeads)
-    {
-        const int ng = (int)min((uint32_t)kScoreHeads, p.G - g0);
-        __syncthreads();
-        for (int g = warp; g < ng; g += kScoreThreads / 32)
-        {
-            const uint16_t *src = p.q + (uint64_t)(s.row0 + i) * p.q_row + (uint64_t)(h * p.G + g0 + g) * p.q_head;
-            float x[D / 32], amax = 0.0f;
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e)
-            {
-                x[e] = kv_float<BF16>(src[lane + 32 * e]);
-                amax = fmaxf(amax, kv_finite_abs(x[e]));
-            }
-            for (int o = 16; o; o >>= 1)
-                amax = fmaxf(amax, __shfl_xor_sync(kKvFull, amax, o));
-            const float qs = kv_scale_of(amax), inv = kv_inverse(qs);
-            int sum = 0;
-            int8_t *dst = reinterpret_cast<int8_t *>(c_s[g]);
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e)
-            {
-                const int c = kv_code(x[e], inv);
-                sum += c;
-                dst[lane + 32 * e] = (int8_t)min(c, 0);
-                dst[D + lane + 32 * e] = (int8_t)max(c, 0);
-            }
-            for (int o = 16; o; o >>= 1)
-                sum += __shfl_xor_sync(kKvFull, sum, o);
-            if (lane == 0)
-            {
-                qs_s[g] = qs;
-                sum_s[g] = sum;
-            }
-        }
-        __syncthreads();
-        for (int g = 0; g < ng; ++g)
-        {
-            int dot = 0;
-            const uint4 *c = reinterpret_cast<const uint4 *>(c_s[g]);
-#pragma unroll
-            for (int e = 0; e < D / 8; ++e)
-            {
-                const uint4 y = c[e];
-                asm("dp4a.u32.s32 %0, %1, %2, %0;" : "+r"(dot) : "r"(w[e].x), "r"(y.x));
-                asm("dp4a.u32.s32 %0, %1, %2, %0;" : "+r"(dot) : "r"(w[e].y), "r"(y.y));
-                asm("dp4a.u32.s32 %0, %1, %2, %0;" : "+r"(dot) : "r"(w[e].z), "r"(y.z));
-                asm("dp4a.u32.s32 %0, %1, %2, %0;" : "+r"(dot) : "r"(w[e].w), "r"(y.w));
-            }
-            best = fmaxf(best, __fmul_rn((float)(dot - 128 * sum_s[g]), qs_s[g]));
-        }
-    }
-    if (j < nb)
-        p.scores[((uint64_t)(s.row0 + i) * p.c.hkv + h) * p.nblk + j] = blk >= 0 ? __fmul_rn(best, ks) : kKvNegInf;
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};\n"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Order-preserving key of a score; larger is better, blocks that are always
-// taken come first.
+// Bytes of a query row in shared memory: 2 D codes, padded so that two rows
+// of 64 bytes lie on different banks.
+template <int D>
+constexpr int code_stride()
+{
+    return (2 * D) % 128 == 64 ? 2 * D : 2 * D + 64;
+}
+
+// Scores of 8 * NT rows of one sequence and one key/value head against
+// `passes` runs of 128 blocks.  Blocks lie on the 16-row side of the matrix
+// instruction, the rows of one query head on its 8-column side, so that the
+// maximum over the query heads stays in the accumulator's lane.  A warp keeps
+// the bounds of its 32 blocks in registers through all heads and rows; a lane
+// takes adjacent bytes, the order of the channels in the sum being free.
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(kScoreThreads) scores_kernel(SelectParams p)
+{
+    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int kRows = 8 * NT, kStride = code_stride<D>(), kChunks = 2 * D / 64;
+    float *qs_s = reinterpret_cast<float *>(smem + p.slots * kRows * kStride);
+    int *init_s = reinterpret_cast<int *>(qs_s + p.slots * kRows);
+    const uint32_t b = blockIdx.z, h = blockIdx.y;
+    const int tile = (int)(blockIdx.x % p.row_tiles), i0 = tile * kRows;
+    const int jbeg = (int)(blockIdx.x / p.row_tiles) * (int)p.passes * kScoreBlocks;
+    const KvSeq s = kv_seq(p.c, b, p.rows);
+    if (i0 >= s.rows)
+        return;
+    const int i1 = min(i0 + kRows, s.rows);
+    const int seen = min(s.first + i1, s.len);
+    const int nb = (max(seen, 0) + (1 << p.c.shift) - 1) >> p.c.shift;
+    const int jend = min(jbeg + (int)p.passes * kScoreBlocks, nb);
+    if (jbeg >= nb)
+        return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+    for (int j0 = jbeg; j0 < jend; j0 += kScoreBlocks)
+    {
+        uint32_t w[2][2][4 * kChunks]; // bounds of blocks (tile, g or g + 8)
+        float ks[2][2];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+            {
+                const int j = j0 + warp * 32 + mt * 16 + u * 8 + g;
+                const int blk = j < jend ? kv_block(p.c, b, j) : -1;
+                const uint64_t si = (uint64_t)max(blk, 0) * p.c.hkv + h;
+                const uint4 *src = reinterpret_cast<const uint4 *>(p.c.bounds + si * 2 * D) + t;
+#pragma unroll
+                for (int i = 0; i < kChunks; ++i)
+                    *reinterpret_cast<uint4 *>(&w[mt][u][4 * i]) =
+                        blk >= 0 ? __ldg(src + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+                ks[mt][u] = blk >= 0 ? __ldg(p.c.ks + si) : -1.0f;
+            }
+        float best[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                best[mt][n][0] = best[mt][n][1] = best[mt][n][2] = best[mt][n][3] = kKvNegInf;
+        for (uint32_t g0 = 0; g0 < p.G; g0 += kScoreHeads)
+        {
+            const int ng = (int)min((uint32_t)kScoreHeads, p.G - g0);
+            if (j0 == jbeg || p.G > kScoreHeads)
+            {
+                __syncthreads();
+                // queries in 8 bits: eight lanes a row, c- (which meets the lower bounds) before c+
+                for (int e = threadIdx.x >> 3; e < ng * kRows; e += kScoreThreads / 8)
+                {
+                    const int hd = e / kRows, i = i0 + e % kRows, l8 = threadIdx.x & 7;
+                    const bool live = i < i1;
+                    const uint16_t *src = p.q + (uint64_t)(s.row0 + (live ? i : i0)) * p.q_row +
+                                          (uint64_t)(h * p.G + g0 + hd) * p.q_head + l8 * (D / 8);
+                    float x[D / 8], amax = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < D / 8; ++k)
+                    {
+                        x[k] = live ? kv_float<BF16>(__ldg(src + k)) : 0.0f;
+                        amax = fmaxf(amax, kv_finite_abs(x[k]));
+                    }
+                    const unsigned eight = 0xFFu << (threadIdx.x & 24);
+                    for (int o = 4; o; o >>= 1)
+                        amax = fmaxf(amax, __shfl_xor_sync(eight, amax, o));
+                    const float qs = kv_scale_of(amax), inv = kv_inverse(qs);
+                    int sum = 0;
+                    uint8_t *dst = smem + (hd * kRows + e % kRows) * kStride + l8 * (D / 8);
+#pragma unroll
+                    for (int k = 0; k < D / 8; k += 4)
+                    {
+                        uint32_t lo = 0u, hi = 0u;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+                        {
+                            const int c = kv_code(x[k + y], inv);
+                            sum += c;
+                            lo |= ((uint32_t)min(c, 0) & 255u) << (8 * y);
+                            hi |= (uint32_t)max(c, 0) << (8 * y);
+                        }
+                        *reinterpret_cast<uint32_t *>(dst + k) = lo;
+                        *reinterpret_cast<uint32_t *>(dst + D + k) = hi;
+                    }
+                    for (int o = 4; o; o >>= 1)
+                        sum += __shfl_xor_sync(eight, sum, o);
+                    if (l8 == 0)
+                    {
+                        qs_s[hd * kRows + e % kRows] = qs;
+                        init_s[hd * kRows + e % kRows] = -128 * sum;
+                    }
+                }
+                __syncthreads();
+            }
+            for (int hd = 0; hd < ng; ++hd)
+            {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                {
+                    const int r = hd * kRows + 8 * n;
+                    const uint8_t *src = smem + (r + g) * kStride + t * 16;
+                    const int2 init = *reinterpret_cast<const int2 *>(init_s + r + 2 * t);
+                    const float2 qs = *reinterpret_cast<const float2 *>(qs_s + r + 2 * t);
+                    int acc[2][4];
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt)
+                    {
+                        acc[mt][0] = acc[mt][2] = init.x;
+                        acc[mt][1] = acc[mt][3] = init.y;
+                    }
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i)
+                    {
+                        const uint4 q = *reinterpret_cast<const uint4 *>(src + 64 * i);
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt)
+                        {
+                            mma_u8s8(acc[mt], w[mt][0][4 * i], w[mt][1][4 * i], w[mt][0][4 * i + 1],
+                                     w[mt][1][4 * i + 1], q.x, q.y);
+                            mma_u8s8(acc[mt], w[mt][0][4 * i + 2], w[mt][1][4 * i + 2], w[mt][0][4 * i + 3],
+                                     w[mt][1][4 * i + 3], q.z, q.w);
+                        }
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            best[mt][n][k] =
+                                fmaxf(best[mt][n][k], __fmul_rn((float)acc[mt][k], k & 1 ? qs.y : qs.x));
+                }
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                {
+                    const int i = i0 + 8 * n + 2 * t + (k & 1);
+                    const int j = j0 + warp * 32 + mt * 16 + (k >> 1) * 8 + g;
+                    const float f = ks[mt][k >> 1];
+                    if (i < i1 && j < jend)
+                        p.scores[((uint64_t)(s.row0 + i) * p.c.hkv + h) * p.width + j] =
+                            f >= 0.0f ? __fmul_rn(best[mt][n][k], f) : kKvNegInf;
+                }
+    }
+}
+
+// Order-preserving key of a score (-0 counts as 0).
 __device__ __forceinline__ uint32_t score_key(float x)
 {
-    const uint32_t u = __float_as_uint(x + 0.0f); // -0 counts as 0
+    const uint32_t u = __float_as_uint(x + 0.0f);
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
+// One thread block per (row, head).  The keys' range is cut into 2048 equal
+// bins; the bin in which the count from above passes what is still needed is
+// cut again until it is taken whole or holds one value (three cuts at most).
+// Equal cuts of the actual range fill more bins than digits of the key would,
+// whose leading bits hardly differ: fewer shared-memory atomics meet.
+template <bool SHARED>
 __global__ void __launch_bounds__(kChooseThreads) choose_kernel(SelectParams p)
 {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t s_digit, s_need;
-    __shared__ uint32_t s_cnt[2][kChooseThreads / 32];
+    extern __shared__ uint32_t keys_s[];
+    __shared__ uint32_t hist[kBins];
+    __shared__ uint32_t s_red[2][kChooseThreads / 32];
+    __shared__ uint32_t s_bin, s_need, s_count;
+    __shared__ uint64_t s_scan[kChooseThreads / 32];
     const uint32_t b = blockIdx.y, h = blockIdx.x % p.c.hkv;
     const int i = (int)(blockIdx.x / p.c.hkv), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const KvSeq s = kv_seq(p.c, b, p.rows);
     if (i >= s.rows)
         return;
     const uint64_t rh = (uint64_t)(s.row0 + i) * p.c.hkv + h;
-    const float *sc = p.scores + rh * p.nblk;
     int32_t *out = p.out + rh * p.select;
     const int seen = min(s.first + i + 1, s.len);
     const int nb = min((max(seen, 0) + (1 << p.c.shift) - 1) >> p.c.shift, (int)p.nblk);
@@ -152,85 +255,123 @@ __global__ void __launch_bounds__(kChooseThreads) choose_kernel(SelectParams p)
             out[e] = e < nb ? e : -1;
         return;
     }
-    const int lo = (int)p.first, hi = nb - (int)p.last;
-    auto key_of = [&](int j) { return j < lo || j >= hi ? 0xFFFFFFFFu : score_key(__ldg(sc + j)); };
-    uint32_t prefix = 0, need = (uint32_t)k;
-    for (int byte = 3; byte >= 0; --byte)
+    const float *sc = p.scores + rh * p.width;
+    const int lo = (int)p.first, hi = nb - (int)p.last; // the blocks that compete
+    uint32_t need = (uint32_t)(k - (int)p.first - (int)p.last);
+    auto key_of = [&](int j) { return SHARED ? keys_s[j] : score_key(__ldg(sc + j)); };
+
+    uint32_t least = 0xFFFFFFFFu, most = 0u;
+    for (int j = lo + tid; j < hi; j += kChooseThreads)
     {
-        for (int e = tid; e < 256; e += kChooseThreads)
-            hist[e] = 0u;
-        __syncthreads();
-        for (int j = tid; j < nb; j += kChooseThreads)
+        const uint32_t key = score_key(__ldg(sc + j));
+        if (SHARED)
+            keys_s[j] = key;
+        least = min(least, key);
+        most = max(most, key);
+    }
+    for (int e = tid; e < kBins; e += kChooseThreads)
+        hist[e] = 0u;
+    least = __reduce_min_sync(kKvFull, least);
+    most = __reduce_max_sync(kKvFull, most);
+    if (lane == 0)
+    {
+        s_red[0][warp] = least;
+        s_red[1][warp] = most;
+    }
+    __syncthreads();
+    for (int w = 0; w < kChooseThreads / 32; ++w)
+    {
+        least = min(least, s_red[0][w]);
+        most = max(most, s_red[1][w]);
+    }
+    // taken: keys above `top`; of the keys in [least, top] the first `need` in block order
+    uint32_t top = need ? most : 0xFFFFFFFFu;
+    if (!need)
+        least = 0xFFFFFFFFu;
+    while (need)
+    {
+        const uint32_t span = top - least;
+        const int shift = max(0, 21 - __clz(span)); // span >> shift < 2048
+        for (int j = lo + tid; j < hi; j += kChooseThreads)
         {
             const uint32_t key = key_of(j);
-            if (byte == 3 || (key >> (8 * (byte + 1))) == prefix)
-                atomicAdd(&hist[(key >> (8 * byte)) & 255u], 1u);
+            if (key >= least && key <= top)
+                atomicAdd(&hist[(key - least) >> shift], 1u);
         }
         __syncthreads();
-        if (warp == 0)
+        // thread t holds eight bins, the highest bins first
+        uint32_t c[kBins / kChooseThreads], sum = 0;
+#pragma unroll
+        for (int e = 0; e < kBins / kChooseThreads; ++e)
         {
-            // lane holds bins 255 - 8 lane ... downwards; the digit is where the count passes need
-            uint32_t c[8], tot = 0;
+            uint32_t *at = &hist[kBins - 1 - tid * (kBins / kChooseThreads) - e];
+            sum += c[e] = *at;
+            *at = 0u;
+        }
+        uint32_t above = sum;
+        for (int o = 1; o < 32; o <<= 1)
+        {
+            const uint32_t y = __shfl_up_sync(kKvFull, above, o);
+            above += lane >= o ? y : 0u;
+        }
+        if (lane == 31)
+            s_red[0][warp] = above;
+        __syncthreads();
+        above -= sum;
+        for (int w = 0; w < warp; ++w)
+            above += s_red[0][w];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                tot += c[e] = hist[255 - 8 * lane - e];
-            uint32_t above = tot;
-            for (int o = 1; o < 32; o <<= 1)
+        for (int e = 0; e < kBins / kChooseThreads; ++e)
+        {
+            if (above < need && above + c[e] >= need)
             {
-                const uint32_t y = __shfl_up_sync(kKvFull, above, o);
-                above += lane >= o ? y : 0u;
+                s_bin = (uint32_t)(kBins - 1 - tid * (kBins / kChooseThreads) - e);
+                s_need = need - above;
+                s_count = c[e];
             }
-            above -= tot;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-            {
-                if (above < need && above + c[e] >= need)
-                {
-                    s_digit = 255u - 8u * lane - e;
-                    s_need = need - above;
-                }
-                above += c[e];
-            }
+            above += c[e];
         }
         __syncthreads();
-        prefix = (prefix << 8) | s_digit;
         need = s_need;
-        __syncthreads();
+        const uint32_t base = least + (s_bin << shift);
+        top = (uint32_t)min((uint64_t)top, (uint64_t)base + ((1u << shift) - 1u));
+        least = base;
+        if (s_count == need || shift == 0)
+            break;
     }
-    // larger keys all, equal keys the first `need` of them
-    int taken = 0;
-    uint32_t equal = 0;
-    for (int j0 = 0; j0 < nb; j0 += kChooseThreads)
+    __syncthreads();
+
+    // every thread writes a run of blocks, behind what the threads before it write
+    const int per = ((nb + kChooseThreads - 1) / kChooseThreads) | 1;
+    const int ja = min(tid * per, nb), jb = min(ja + per, nb);
+    uint64_t mine = 0; // (keys in [least, top]) << 32 | (keys above, blocks always taken)
+    for (int j = ja; j < jb; ++j)
     {
-        const int j = j0 + tid;
-        const uint32_t key = j < nb ? key_of(j) : 0u;
-        const bool gt = j < nb && key > prefix, eq = j < nb && key == prefix;
-        const uint32_t mg = __ballot_sync(kKvFull, gt), me = __ballot_sync(kKvFull, eq);
-        if (lane == 0)
-        {
-            s_cnt[0][warp] = __popc(mg);
-            s_cnt[1][warp] = __popc(me);
-        }
-        __syncthreads();
-        uint32_t g_before = 0, e_before = 0, g_all = 0, e_all = 0;
-        for (int w = 0; w < kChooseThreads / 32; ++w)
-        {
-            if (w < warp)
-                g_before += s_cnt[0][w], e_before += s_cnt[1][w];
-            g_all += s_cnt[0][w], e_all += s_cnt[1][w];
-        }
-        const uint32_t below = (1u << lane) - 1u;
-        const uint32_t e_rank = equal + e_before + __popc(me & below);
-        if (gt || (eq && e_rank < need))
-        {
-            const uint32_t at = (uint32_t)taken + g_before + __popc(mg & below) +
-                                min(e_rank, need) - min(equal, need);
-            if (at < (uint32_t)k)
-                out[at] = j;
-        }
-        taken += (int)(g_all + min(equal + e_all, need) - min(equal, need));
-        equal += e_all;
-        __syncthreads();
+        const bool always = j < lo || j >= hi;
+        const uint32_t key = always ? 0u : key_of(j);
+        mine += always || key > top ? 1ull : (need && key >= least ? 1ull << 32 : 0ull);
+    }
+    uint64_t incl = mine;
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const uint64_t y = __shfl_up_sync(kKvFull, incl, o);
+        incl += lane >= o ? y : 0ull;
+    }
+    if (lane == 31)
+        s_scan[warp] = incl;
+    __syncthreads();
+    uint64_t before = incl - mine;
+    for (int w = 0; w < warp; ++w)
+        before += s_scan[w];
+    uint32_t sure = (uint32_t)before, maybe = (uint32_t)(before >> 32);
+    for (int j = ja; j < jb; ++j)
+    {
+        const bool always = j < lo || j >= hi;
+        const uint32_t key = always ? 0u : key_of(j);
+        if (always || key > top)
+            out[min(sure++ + min(maybe, need), (uint32_t)k - 1u)] = j;
+        else if (need && key >= least && maybe++ < need)
+            out[min(sure + maybe - 1u, (uint32_t)k - 1u)] = j;
     }
 }
 
@@ -240,19 +381,45 @@ uint32_t score_blocks(const DanceKvCache &c, const DanceKvBatch &b)
     return (uint32_t)(n < b.table_width ? n : b.table_width);
 }
 
-template <int D>
-int launch_select(const SelectParams &p, bool bf16, cudaStream_t st)
+// Floats from one (row, head)'s scores to the next: whole sectors.
+uint32_t score_width(uint32_t nblk) { return (nblk + 7u) & ~7u; }
+
+template <int D, int NT>
+int launch_scores(SelectParams &p, bool bf16, cudaStream_t st)
 {
-    const dim3 grid((p.nblk + kScoreThreads - 1) / kScoreThreads, p.c.max_rows * p.c.hkv, p.c.batch);
+    p.row_tiles = (p.c.max_rows + 8 * NT - 1) / (8 * NT);
+    const uint32_t runs = (p.nblk + kScoreBlocks - 1) / kScoreBlocks;
+    const uint64_t tiles = (uint64_t)p.row_tiles * p.c.hkv * p.c.batch;
+    // runs of one thread block: one, unless there is work for several waves without
+    p.passes = (uint32_t)(tiles * runs >= 4 * 4 * 148 ? min(4u, runs) : 1u);
+    const dim3 grid(p.row_tiles * ((runs + p.passes - 1) / p.passes), p.c.hkv, p.c.batch);
+    constexpr int per_head = 8 * NT * (code_stride<D>() + 8), most = kScoreHeads * per_head;
+    p.slots = min(p.G, (uint32_t)kScoreHeads);
+    const int smem = (int)p.slots * per_head;
+    static const cudaError_t attr[2] = {
+        cudaFuncSetAttribute(scores_kernel<D, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most),
+        cudaFuncSetAttribute(scores_kernel<D, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)};
+    DANCE_CUDA(attr[0]);
+    DANCE_CUDA(attr[1]);
+    if (bf16)
+        scores_kernel<D, NT, true><<<grid, kScoreThreads, smem, st>>>(p);
+    else
+        scores_kernel<D, NT, false><<<grid, kScoreThreads, smem, st>>>(p);
+    DANCE_LAUNCHED();
+    return 0;
+}
+
+template <int D>
+int launch_select(SelectParams &p, bool bf16, cudaStream_t st)
+{
     if (p.nblk > p.select)
-    {
-        if (bf16)
-            scores_kernel<D, true><<<grid, kScoreThreads, 0, st>>>(p);
-        else
-            scores_kernel<D, false><<<grid, kScoreThreads, 0, st>>>(p);
-        DANCE_LAUNCHED();
-    }
-    choose_kernel<<<dim3(p.c.max_rows * p.c.hkv, p.c.batch), kChooseThreads, 0, st>>>(p);
+        if (int rc = p.c.max_rows <= 8 ? launch_scores<D, 1>(p, bf16, st) : launch_scores<D, 4>(p, bf16, st))
+            return rc;
+    const dim3 grid(p.c.max_rows * p.c.hkv, p.c.batch);
+    if (p.nblk <= kChooseKeys)
+        choose_kernel<true><<<grid, kChooseThreads, p.nblk * 4, st>>>(p);
+    else
+        choose_kernel<false><<<grid, kChooseThreads, 0, st>>>(p);
     DANCE_LAUNCHED();
     return 0;
 }
@@ -261,7 +428,7 @@ int launch_select(const SelectParams &p, bool bf16, cudaStream_t st)
 
 uint64_t kv_select_bytes(const DanceKvCache &c, const DanceKvBatch &b, uint32_t rows)
 {
-    return (uint64_t)rows * c.kv_heads * score_blocks(c, b) * 4u;
+    return (uint64_t)rows * c.kv_heads * score_width(score_blocks(c, b)) * 4u;
 }
 uint64_t kv_attention_bytes(const DanceKvCache &c, const DanceKvBatch &b, uint32_t heads, uint32_t select);
 uint64_t kv_counter_bytes();
@@ -301,6 +468,7 @@ extern "C" int dance_kv_select_blocks(const DanceKvCache *cache, const DanceKvBa
     p.heads = num_heads;
     p.G = num_heads / cache->kv_heads;
     p.nblk = score_blocks(*cache, *batch);
+    p.width = score_width(p.nblk);
     p.select = select;
     p.first = first_blocks;
     p.last = last_blocks;
