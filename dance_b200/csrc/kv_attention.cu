@@ -17,7 +17,7 @@
 // the sum of the weights (taken before rounding) and the output.
 #include <cuda_runtime.h>
 
-#include "kv_common.cuh"
+#include "kv_attention.cuh"
 
 namespace dance
 {
@@ -25,33 +25,10 @@ namespace
 {
 
 constexpr int kWarps = 4;
-constexpr int kTile = 32;        // tokens of a warp's tile
-constexpr int kStages = 3;       // tiles of a warp in flight or in use
-constexpr int kEntries = 512;    // cache blocks looked up at once
-constexpr float kBoost = 14.0f;  // log2 of what a weight of 1 is as a half
-constexpr uint32_t kCounters = 1u << 16;
-constexpr int kMaxPos = 0x3FFFFFFF;
-
-struct AttnParams
-{
-    KvView c;
-    const uint16_t *q;
-    uint64_t q_row, q_head;
-    uint32_t rows, heads, G;
-    bool q_aligned;
-    float scale_log2;
-    const int32_t *blocks; // sparse: rows x hkv x select
-    uint32_t select;
-    uint32_t chunk;     // cache blocks of one split
-    uint32_t splits;    // most splits of a sequence
-    uint32_t row_tiles; // row tiles of a (sequence or row, head)
-    void *out;
-    float *lse;
-    uint32_t *counters;
-    float *part; // partial outputs, then partial log-sums
-};
-
-__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+constexpr int kTile = 32;       // tokens of a warp's tile
+constexpr int kStages = 3;      // tiles of a warp in flight or in use
+constexpr int kEntries = 512;   // cache blocks looked up at once
+constexpr float kBoost = 14.0f; // log2 of what a weight of 1 is as a half
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src)
 {
@@ -79,22 +56,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x)
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
-}
-
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Two bytes of w (sel 0x4140: the low two, 0x4342: the high two) as the
-// halves c - 128.
-__device__ __forceinline__ uint32_t code_halves(uint32_t w, uint32_t sel)
-{
-    const uint32_t u = __byte_perm(w, 0x64646464u, sel);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t *>(&r);
 }
 
 // Byte offset of 16-byte chunk ch of a tile's token in shared memory.  Keys
@@ -250,11 +211,8 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
             amax = fmaxf(amax, fabsf(x[e]));
         amax = fmaxf(amax, __shfl_xor_sync(kKvFull, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(kKvFull, amax, 2));
-        // 2^(13 - exponent): the largest channel lands in [2^13, 2^14)
-        const int ex = (int)(__float_as_uint(amax) >> 23);
-        const int up = (ex == 255 || amax == 0.0f) ? 0 : min(126, 127 + 13 - ex);
-        const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
-        const float back = __uint_as_float((uint32_t)(127 - up) << 23);
+        const int up = row_shift(amax);
+        const float mul = power_of_two(up), back = power_of_two(-up);
 #pragma unroll
         for (int e = 0; e < 2 * kSteps; ++e)
             qf[j][e] = live ? kv_pack<false>(x[2 * e] * mul, x[2 * e + 1] * mul) : 0u;
@@ -629,41 +587,55 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
     }
 }
 
-// How a call is cut: rows of a tile, splits, workspace.
-struct AttnPlan
-{
-    uint32_t nt, row_tiles, chunk, splits;
-    uint64_t items, blocks_x, bytes;
-};
+constexpr uint32_t kSlots = 2 * 148;       // blocks of rows_kernel that the GPU holds at once
+constexpr uint32_t kPromptSlots = 148;     // blocks of the kernel of many rows
+constexpr uint64_t kPromptLeast = 32;      // rows of a sequence and key/value head from which it is used
 
-constexpr uint32_t kSlots = 2 * 148; // blocks of rows_kernel that the GPU holds at once
-
-AttnPlan plan_rows(const DanceKvCache &c, const DanceKvBatch &b, uint32_t heads, uint32_t select)
+AttnPlan plan_attention(const DanceKvCache &c, const DanceKvBatch &b, uint32_t heads, uint32_t select)
 {
     AttnPlan a;
     const uint32_t G = heads / c.kv_heads;
     const uint64_t rows = select ? G : (uint64_t)b.max_rows * G;
+    a.prompt = !select && rows > kPromptLeast;
     a.nt = rows <= 8 ? 1u : 2u;
-    a.row_tiles = (uint32_t)((rows + 8 * a.nt - 1) / (8 * a.nt));
+    const uint32_t tile = a.prompt ? kPromptRows : 8 * a.nt;
+    a.row_tiles = (uint32_t)((rows + tile - 1) / tile);
     const uint64_t per_b = (uint64_t)c.kv_heads * a.row_tiles * (select ? b.max_rows : 1u);
-    a.items = per_b * b.batch;
-    const uint64_t len = b.max_len < (uint64_t)b.table_width * c.block_tokens ? b.max_len
-                                                                             : (uint64_t)b.table_width * c.block_tokens;
+    const uint64_t items = per_b * b.batch;
+    const uint64_t cap = (uint64_t)b.table_width * c.block_tokens;
+    const uint64_t len = b.max_len < cap ? b.max_len : cap;
     const uint32_t ent = select ? select : (uint32_t)((len + c.block_tokens - 1) / c.block_tokens);
-    // splits: about four waves of blocks, none under 256 tokens
-    uint64_t want = (4 * kSlots + a.items - 1) / (a.items ? a.items : 1);
-    const uint64_t most = ((uint64_t)ent * c.block_tokens + 255) / 256;
-    want = want > most ? most : want;
-    if (want < 1 || a.items > kCounters)
+    const uint64_t tokens = (uint64_t)ent * c.block_tokens;
+    uint64_t want = 1;
+    uint32_t unit = c.block_tokens == 16 ? 2 : 1; // cache blocks of a tile of 32 tokens
+    if (a.prompt)
+    {
+        // splits: as many as fill the last wave best, none under 512 tokens
+        unit = c.block_tokens < kPromptTokens ? kPromptTokens / c.block_tokens : 1;
+        double best = 1e30;
+        for (uint64_t s = 1; s <= kPromptSlots && (s == 1 || tokens / s >= 512); ++s)
+        {
+            const double waves = (double)((items * s + kPromptSlots - 1) / kPromptSlots) / (double)s;
+            const double cost = waves * (double)tokens + (s > 1 ? 256.0 : 0.0) + 16.0 * (double)s;
+            if (cost < best)
+                best = cost, want = s;
+        }
+    }
+    else
+    {
+        // about four waves of blocks, none under 256 tokens
+        want = (4 * kSlots + items - 1) / (items ? items : 1);
+        const uint64_t most = (tokens + 255) / 256;
+        want = want > most ? most : want;
+    }
+    if (want < 1 || items > kCounters)
         want = 1;
     a.chunk = (uint32_t)((ent + want - 1) / want);
-    if (c.block_tokens == 16)
-        a.chunk += a.chunk & 1u;
-    a.chunk = a.chunk ? a.chunk : 1;
+    a.chunk = a.chunk ? (a.chunk + unit - 1) / unit * unit : unit;
     a.splits = (ent + a.chunk - 1) / a.chunk;
     a.splits = a.splits ? a.splits : 1;
     a.blocks_x = per_b * a.splits;
-    a.bytes = kCounters * 4ull + (a.splits > 1 ? a.items * a.splits * 8 * a.nt * (c.head_dim + 1) * 4ull : 0ull);
+    a.bytes = kCounters * 4ull + (a.splits > 1 ? items * a.splits * tile * (c.head_dim + 1) * 4ull : 0ull);
     return a;
 }
 
@@ -717,7 +689,7 @@ int attend(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRo
         return 0;
     if (!d_out || (uintptr_t)d_out % 16 || (uintptr_t)d_lse % 4)
         return fail(-1, "null or misaligned output");
-    const AttnPlan a = plan_rows(*cache, *batch, num_heads, select);
+    const AttnPlan a = plan_attention(*cache, *batch, num_heads, select);
     if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < a.bytes)
         return fail(-1, "workspace of %llu bytes: %llu are needed", (unsigned long long)workspace_bytes,
                     (unsigned long long)a.bytes);
@@ -744,6 +716,8 @@ int attend(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRo
     p.part = reinterpret_cast<float *>(p.counters + kCounters);
     const dim3 grid((unsigned)a.blocks_x, batch->batch);
     const bool bf16 = q->dtype == DANCE_BF16;
+    if (a.prompt)
+        return launch_prompt(p, cache->head_dim, bf16, (uint32_t)a.blocks_x, as_stream(stream));
     switch (cache->head_dim)
     {
     case 64:
@@ -760,7 +734,7 @@ int attend(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRo
 uint64_t kv_counter_bytes() { return kCounters * 4ull; }
 uint64_t kv_attention_bytes(const DanceKvCache &c, const DanceKvBatch &b, uint32_t heads, uint32_t select)
 {
-    return plan_rows(c, b, heads, select).bytes;
+    return plan_attention(c, b, heads, select).bytes;
 }
 
 } // namespace dance
