@@ -610,13 +610,14 @@ AttnPlan plan_attention(const DanceKvCache &c, const DanceKvBatch &b, uint32_t h
     uint32_t unit = c.block_tokens == 16 ? 2 : 1; // cache blocks of a tile of 32 tokens
     if (a.prompt)
     {
-        // splits: as many as fill the last wave best, none under 512 tokens
+        // splits: what fills the waves of blocks best, a block's start and end counting like 768 tokens,
+        // the joining of splits like 768 more
         unit = c.block_tokens < kPromptTokens ? kPromptTokens / c.block_tokens : 1;
-        double best = 1e30;
+        uint64_t best = ~0ull;
         for (uint64_t s = 1; s <= kPromptSlots && (s == 1 || tokens / s >= 512); ++s)
         {
-            const double waves = (double)((items * s + kPromptSlots - 1) / kPromptSlots) / (double)s;
-            const double cost = waves * (double)tokens + (s > 1 ? 256.0 : 0.0) + 16.0 * (double)s;
+            const uint64_t cost = (items * s + kPromptSlots - 1) / kPromptSlots *
+                                  (tokens / s + (s > 1 ? 1536u : 768u));
             if (cost < best)
                 best = cost, want = s;
         }

@@ -8,15 +8,27 @@
 //   P = weights (softmax threads: S from tensor memory, P back over it as f16)
 //   O += P V    (A = P from tensor memory, B in shared memory)
 // The two row tiles alternate, so that the tensor core works on one while the
-// softmax threads work on the other; tensor memory is full: 2 x 128 columns of
-// S (P lies over the first half of its S) and 2 x head_dim of O.
+// softmax threads work on the other.  Tensor memory is full: 2 x 128 columns
+// of S (P lies over the first half of its S) and 2 x head_dim of O.
+//
+// Measured on 2594 rows x 32 heads over 16000 and 7100 tokens of 128 channels:
+// 0.82 ms, 0.69 PFLOP/s (0.41 of the measured matrix rate).  What bounds it is
+// the chain softmax -> P V -> Q K^T of each row tile, about 5300 clocks for
+// 128 tokens where the tensor core works 2100: tensor core, exponentials and
+// issue slots are each under half used.  Tried and slower, from 0.88 to 0.90
+// ms: scores in two buffers of 64 columns computed ahead, 0.94 (a product of
+// 64 columns takes the tensor core as long as one of 128); weights handed over
+// in halves, 0.95; a quarter of the exponentials as polynomials, 0.95.  What
+// helped: the row's logits read from tensor memory once, 1.21 -> 0.88 together
+// with registers handed to the softmax threads; one short copy of the code
+// that issues the products (it competes with long unrolled loops for the
+// instruction cache), 0.90 -> 0.86.
 //
 // Warps 0-3 and 4-7 hold the rows' softmax, one thread per row and no exchange
 // between threads.  Warps 8-11 turn codes into halves: a tile's raw bytes are
-// loaded into registers one tile ahead, then converted and stored in the
-// K-major core-matrix layout (8 rows x 16 bytes); the same layout read as
-// MN-major serves V, whose rows are the summed dimension.  Warp 12 issues the
-// matrix instructions.
+// loaded into registers one tile ahead, then converted and stored, a token a
+// row, with a 128-byte swizzle; K is read as K-major, V, whose rows are the
+// summed dimension, as MN-major.  Warp 12 issues the matrix instructions.
 //
 // Rescaling O in tensor memory is a round trip, so a row keeps its reference
 // maximum until the true one exceeds it by 2^8: weights are 2^(s - ref + 7) <=
@@ -25,6 +37,8 @@
 // Every wait on a barrier is bounded.  A block that gives up counts itself in
 // g_kv_prompt_timeouts, and its rows read as not-a-number.
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "kv_attention.cuh"
 
@@ -38,25 +52,31 @@ namespace
 {
 
 constexpr int kSoftWarps = 8, kConvWarps = 4;
-constexpr int kThreads = 32 * (kSoftWarps + kConvWarps + 1);
+constexpr int kMmaWarp = kSoftWarps + kConvWarps;
+// Four groups of four warps, so that registers can be handed between them (the
+// last group's other warps only wait): 128 x (2 x 192 + 80 + 48) = 512 x 128.
+constexpr int kThreads = 512;
+constexpr int kSoftRegs = 192, kConvRegs = 80, kMmaRegs = 48;
 constexpr int kTok = (int)kPromptTokens;
 constexpr int kGroups = kTok / 16;    // 16 tokens share a cache block
 constexpr int kFactorStages = 4;      // factors are read up to two tiles after the codes are free
 constexpr float kLift = 7.0f;         // log2 of the weight of a row's reference maximum
 constexpr float kSlack = 8.0f;        // how far the maximum may rise above the reference
-constexpr uint32_t kWaitLimit = 1u << 24;
+constexpr uint32_t kWaitNs = 20000;       // how long one try may sleep
+constexpr uint32_t kWaitLimit = 1u << 16; // tries
 
 template <int D>
 struct Layout
 {
-    static constexpr int kTileBytes = kTok * D * 2; // 128 rows of D halves
+    static constexpr int kTileBytes = (D + 63) / 64 * kTok * 128; // 128 rows of halves, 64 channels a run of 16 KB
     static constexpr int q = 0;                     // two row tiles
     static constexpr int k = 2 * kTileBytes;        // two stages
     static constexpr int v = 4 * kTileBytes;        // two stages
-    static constexpr int factors = 6 * kTileBytes;  // kFactorStages x kGroups x (logit, weight, position, -)
+    static constexpr int factors = 6 * kTileBytes;  // kFactorStages x kGroups x (logit factor, log2 of the
+                                                    // weight's factor, position, its inverse)
     static constexpr int bars = factors + kFactorStages * kGroups * 16;
-    static constexpr int misc = bars + 16 * 8;
-    static constexpr int used = misc + 64;
+    static constexpr int misc = bars + 24 * 8;
+    static constexpr int used = misc + 64 + 1024;
     // more than half of an SM's shared memory: a second block would wait for tensor memory
     static constexpr int bytes = used > 118 * 1024 ? used : 118 * 1024;
 };
@@ -67,11 +87,10 @@ enum Bar : int
     kVFull = 2,
     kKEmpty = 4,
     kVEmpty = 6,
-    kSFull = 8, // 2 row tiles
+    kSFull = 8,  // 2 row tiles
     kPFull = 10,
     kODone = 12,
-    kDrain = 14,
-    kBars = 15
+    kDrain = 14
 };
 
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count)
@@ -85,10 +104,10 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar)
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
 {
     uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
                  "selp.u32 %0, 1, 0, p;\n\t}\n"
                  : "=r"(ok)
-                 : "r"(bar), "r"(parity)
+                 : "r"(bar), "r"(parity), "r"(kWaitNs)
                  : "memory");
     return ok != 0;
 }
@@ -101,7 +120,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     {
         if (bar_try(bar, parity))
             return true;
-        if ((it & 255u) == 255u && *gave_up)
+        if ((it & 15u) == 15u && *gave_up)
             return false;
     }
     *gave_up = 1;
@@ -111,38 +130,67 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-// Shared-memory matrix descriptor without swizzle: start, leading and stride
-// byte offsets, descriptor version 1.  K-major: leading = from one 16-byte
-// column of core matrices to the next, stride = from 8 rows to the next 8.
-// MN-major: leading = from 8 rows (of the summed dimension) to the next 8,
-// stride = from one 16-byte column to the next.
+// Shared-memory matrix descriptor with 128-byte swizzle: start, leading and
+// stride byte offsets, descriptor version 1.  K-major: stride = from 8 rows to
+// the next 8 (leading unused).  MN-major: leading = from 64 channels to the
+// next 64, stride = from 8 rows (of the summed dimension) to the next 8.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride)
 {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)((leading >> 4) & 0x3FFFu) << 16) |
-           ((uint64_t)((stride >> 4) & 0x3FFFu) << 32) | (1ull << 46);
+           ((uint64_t)((stride >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
 }
 // kind::f16 instruction descriptor: f32 sums, f16 operands, M = 128.
 constexpr uint32_t instr_desc(int n, bool b_mn_major)
 {
     return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+// The products of one tile, issued in one go by the lane with `leader`; of the
+// descriptors only the low words, which hold the start in 16 bytes, advance.
+// S = Q K^T over D channels: 16 channels are 32 bytes of a row, 64 a run.
+template <int D>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, uint32_t leader)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                 : "memory");
+#define DANCE_SS(at, acc)                                                                                        \
+    "add.u32 u, %1, " #at ";\n\tadd.u32 v, %2, " #at ";\n\tmov.b64 x, {u, %5};\n\tmov.b64 y, {v, %5};\n\t"         \
+    "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, " #acc ";\n\t"
+#define DANCE_SS_HEAD                                                                                            \
+    "{\n\t.reg .pred n, p, q;\n\t.reg .b64 x, y;\n\t.reg .b32 u, v;\n\tsetp.ne.b32 q, %4, 0;\n\t"                 \
+    "setp.ne.b32 n, %4, %4;\n\tsetp.eq.b32 p, %4, %4;\n\t"                                                      \
+    DANCE_SS(0, n) DANCE_SS(2, p) DANCE_SS(4, p) DANCE_SS(6, p)
+    static_assert(kTok * 8 == 1024, "offset of the second run");
+    if constexpr (D == 128)
+        asm volatile(DANCE_SS_HEAD DANCE_SS(1024, p) DANCE_SS(1026, p) DANCE_SS(1028, p) DANCE_SS(1030, p) "}\n" ::"r"(d),
+                     "r"(a), "r"(b), "r"(idesc), "r"(leader), "r"(high)
+                     : "memory");
+    else if constexpr (D == 96)
+        asm volatile(DANCE_SS_HEAD DANCE_SS(1024, p) DANCE_SS(1026, p) "}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+                     "r"(leader), "r"(high)
+                     : "memory");
+    else
+        asm volatile(DANCE_SS_HEAD "}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(leader), "r"(high) : "memory");
+#undef DANCE_SS_HEAD
+#undef DANCE_SS
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+// O (+)= P V over 128 tokens: 16 tokens are 8 columns of P and 2 KB of V.
+__device__ __forceinline__ void mma_values(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc,
+                                           uint32_t accumulate, uint32_t leader)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+#define DANCE_TS(col, at, acc)                                                                                   \
+    "add.u32 x, %1, " #col ";\n\tadd.u32 v, %2, " #at ";\n\tmov.b64 y, {v, %6};\n\t"                             \
+    "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, " #acc ";\n\t"
+    asm volatile("{\n\t.reg .pred n, p, q;\n\t.reg .b32 x, v;\n\t.reg .b64 y;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "setp.ne.b32 n, %4, 0;\n\tsetp.eq.b32 p, %4, %4;\n\t" DANCE_TS(0, 0, n) DANCE_TS(8, 128, p)
+                     DANCE_TS(16, 256, p) DANCE_TS(24, 384, p) DANCE_TS(32, 512, p) DANCE_TS(40, 640, p)
+                         DANCE_TS(48, 768, p) DANCE_TS(56, 896, p) "}\n" ::"r"(d),
+                 "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(leader), "r"(high)
                  : "memory");
+#undef DANCE_TS
 }
-__device__ __forceinline__ void commit(uint32_t bar)
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t leader)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar)
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar),
+                 "r"(leader)
                  : "memory");
 }
 
@@ -158,7 +206,49 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32])
                    "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(addr));
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+                 "%13, %14, %15}, [%16];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+}
+// Waits for the loads in flight; what they loaded passes through, so that no
+// use of it can move ahead of the wait.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                   "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void loaded(uint32_t (&r)[32])
+{
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                   "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
 {
@@ -168,18 +258,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
                  "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-                 "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-                 "%32};\n" ::"r"(addr),
-                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-                 "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-                 "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-                 : "memory");
-}
-
 // Two floats in one register pair: one instruction for both.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 {
@@ -190,30 +268,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+// Byte offset of 16-byte chunk c (8 channels) of row r: runs of 64 channels,
+// 128 bytes a row, the chunks of eight rows exchanged (128-byte swizzle) so
+// that neither the threads that store a column of rows nor the tensor core
+// that reads one meet on a bank.
+__device__ __forceinline__ uint32_t tile_off(int r, int c)
 {
-    float2 r;
-    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-        "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}\n"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
-{
-    float2 r;
-    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}\n"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-
-// Byte offset of 16-byte chunk c of row r in the core-matrix layout.
-template <int D>
-__device__ __forceinline__ uint32_t core_off(int r, int c)
-{
-    return (uint32_t)((r >> 3) * (D / 8 * 128) + c * 128 + (r & 7) * 16);
+    return (uint32_t)((c >> 3) * (kTok * 128) + r * 128 + (((c ^ r) & 7) << 4));
 }
 
 // What a block works on.
@@ -231,7 +292,8 @@ struct Work
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
 {
-    extern __shared__ __align__(1024) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((0u - smem_addr(smem_raw)) & 1023u); // the swizzle counts from 1024 bytes
     using L = Layout<D>;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Work w;
@@ -266,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
     uint32_t *s_vmax = reinterpret_cast<uint32_t *>(smem + L::misc + 12);
     float4 *s_f = reinterpret_cast<float4 *>(smem + L::factors);
 
-    if (warp == kSoftWarps + kConvWarps)
+    if (warp == kMmaWarp)
     {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tmem_slot)),
                      "r"(512u)
@@ -346,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             for (int e = 0; e < 4; ++e)
                 y[e] = kv_pack<false>(kv_float<BF16>((uint16_t)x[4 * c + e]) * mul,
                                       kv_float<BF16>((uint16_t)(x[4 * c + e] >> 16)) * mul);
-            *reinterpret_cast<uint4 *>(smem + L::q + (tid >> 7) * L::kTileBytes + core_off<D>(tid & 127, c)) =
+            *reinterpret_cast<uint4 *>(smem + L::q + (tid >> 7) * L::kTileBytes + tile_off(tid & 127, c)) =
                 make_uint4(y[0], y[1], y[2], y[3]);
         }
         rf = live ? power_of_two(-up) * p.scale_log2 : 0.0f;
@@ -361,6 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
     if (warp < kSoftWarps)
     {
         // ------------------------------------------------ softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftRegs));
         const int tile = warp >> 2;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21; // tensor-memory lane in bits 16 and up
         const uint32_t s_addr = tmem + lanes + 128u * (uint32_t)tile;
@@ -378,42 +441,91 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             }
             fence_after();
             const float4 *f = s_f + (i % kFactorStages) * kGroups;
-            const int pos0 = w.base + i * kTok;
-            bool whole = pos0 + kTok <= tile_lo;
+
+            // The row's 128 logits stay in registers from the maximum to the weights.
+            uint32_t x[4][32];
+            tmem_ld32(s_addr, x[0]);
+            tmem_ld32(s_addr + 32u, x[1]);
+            bool whole = w.base + (i + 1) * kTok <= tile_lo;
 #pragma unroll
             for (int g = 0; g < kGroups; ++g)
                 whole &= __float_as_int(f[g].z) != kMaxPos;
-
-            // the tile's maximum; the products' factor is not negative and constant over 16 tokens
+            tmem_ld_wait(x[0]);
+            loaded(x[1]);
+            tmem_ld32(s_addr + 64u, x[2]);
+            tmem_ld32(s_addr + 96u, x[3]);
             float top = kKvNegInf;
+            // the logits' factor is not negative and constant over 16 tokens
+            auto maximum = [&](auto masked, int g0) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-            {
-                uint32_t x[32];
-                tmem_ld32(s_addr + 32u * c, x);
-                tmem_ld_wait();
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int g = g0; g < g0 + kGroups / 2; ++g)
                 {
-                    const int g = 2 * c + u;
                     const float4 fg = f[g];
-                    float gm = kKvNegInf;
-                    if (whole)
-                    {
+                    float m0 = kKvNegInf, m1 = kKvNegInf;
+                    const int left = limit - __float_as_int(fg.z); // columns of the group that the row sees
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            gm = fmaxf(gm, __uint_as_float(x[16 * u + e]));
+                    for (int e = 0; e < 8; ++e)
+                    {
+                        const float y0 = __uint_as_float(x[g >> 1][16 * (g & 1) + e]);
+                        const float y1 = __uint_as_float(x[g >> 1][16 * (g & 1) + e + 8]);
+                        m0 = fmaxf(m0, !masked || e < left ? y0 : kKvNegInf);
+                        m1 = fmaxf(m1, !masked || e + 8 < left ? y1 : kKvNegInf);
                     }
+                    m0 = fmaxf(m0, m1);
+                    if constexpr (masked)
+                        top = fmaxf(top, m0 == kKvNegInf ? kKvNegInf : m0 * (fg.x * rf));
                     else
-                    {
-                        const int left = limit - __float_as_int(fg.z); // columns of the group that the row sees
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            gm = fmaxf(gm, e < left ? __uint_as_float(x[16 * u + e]) : kKvNegInf);
-                    }
-                    top = fmaxf(top, gm == kKvNegInf ? kKvNegInf : gm * (fg.x * rf));
+                        top = fmaxf(top, m0 * (fg.x * rf));
                 }
-            }
+            };
+            auto weights = [&](auto masked, float shift_m) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                {
+                    uint32_t y[16];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                    {
+                        const float4 fg = f[2 * c + u];
+                        const float kf = fg.x * rf, sm = shift_m + fg.y;
+                        const int left = limit - __float_as_int(fg.z);
+                        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                        {
+                            float2 z = fma2(make_float2(__uint_as_float(x[c][16 * u + 2 * e]),
+                                                        __uint_as_float(x[c][16 * u + 2 * e + 1])),
+                                            make_float2(kf, kf), make_float2(sm, sm));
+                            if constexpr (masked)
+                            {
+                                // cut off what the exponent's unrounded product exceeds the maximum by; a logit
+                                // that is not a number stays one
+                                z.x = z.x > kLift + kSlack ? kLift + kSlack : z.x;
+                                z.y = z.y > kLift + kSlack ? kLift + kSlack : z.y;
+                                z.x = 2 * e < left ? z.x : kKvNegInf;
+                                z.y = 2 * e + 1 < left ? z.y : kKvNegInf;
+                            }
+                            z.x = exp2_fast(z.x);
+                            z.y = exp2_fast(z.y);
+                            sum.x += z.x;
+                            sum.y += z.y;
+                            y[8 * u + e] = kv_pack<false>(z.x, z.y);
+                        }
+                        l = fmaf(sum.x + sum.y, fg.w, l);
+                    }
+                    tmem_st16(s_addr + 16u * c, y);
+                }
+            };
+            if (whole)
+                maximum(std::false_type{}, 0);
+            else
+                maximum(std::true_type{}, 0);
+            tmem_ld_wait(x[2]);
+            loaded(x[3]);
+            if (whole)
+                maximum(std::false_type{}, kGroups / 2);
+            else
+                maximum(std::true_type{}, kGroups / 2);
             const bool rise = top > m + kSlack; // from -inf: any maximum
             if (__any_sync(kKvFull, rise))
             {
@@ -422,62 +534,26 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 l *= down;
                 if (i > 0)
                 {
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c)
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c)
                     {
-                        uint32_t x[32];
-                        tmem_ld32(o_addr + 32u * c, x);
-                        tmem_ld_wait();
+                        uint32_t o[16];
+                        tmem_ld16(o_addr + 16u * c, o);
+                        tmem_ld_wait(o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
-                        tmem_st32(o_addr + 32u * c, x);
+                        for (int e = 0; e < 16; ++e)
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) * down);
+                        tmem_st16(o_addr + 16u * c, o);
                     }
                 }
             }
             const float shift_m = m == kKvNegInf ? 0.0f : kLift - m;
-            // the exponent's product is not rounded where the maximum's was: beyond 2^20 that difference shows,
-            // and is cut off
+            // the exponent's product is not rounded where the maximum's was: beyond 2^20 that difference shows
             const bool plain = whole && __all_sync(kKvFull, fabsf(m) < 1048576.0f);
-            float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-            {
-                uint32_t x[32], y[16];
-                tmem_ld32(s_addr + 32u * c, x);
-                tmem_ld_wait();
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                {
-                    const float4 fg = f[2 * c + u];
-                    const float kf = fg.x * rf;
-                    const int left = plain ? 16 : limit - __float_as_int(fg.z);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                    {
-                        float2 z = fma2(make_float2(__uint_as_float(x[16 * u + 2 * e]), __uint_as_float(x[16 * u + 2 * e + 1])),
-                                        make_float2(kf, kf), make_float2(shift_m, shift_m));
-                        if (!plain)
-                        {
-                            // a logit that is not a number stays one
-                            z.x = z.x > kLift + kSlack ? kLift + kSlack : z.x;
-                            z.y = z.y > kLift + kSlack ? kLift + kSlack : z.y;
-                        }
-                        z.x = exp2_fast(z.x);
-                        z.y = exp2_fast(z.y);
-                        if (!plain)
-                        {
-                            z.x = 2 * e < left ? z.x : 0.0f;
-                            z.y = 2 * e + 1 < left ? z.y : 0.0f;
-                        }
-                        sum = add2(sum, z);
-                        z = mul2(z, make_float2(fg.y, fg.y));
-                        y[8 * u + e] = kv_pack<false>(z.x, z.y);
-                    }
-                }
-                tmem_st16(s_addr + 16u * c, y);
-            }
-            l += sum.x + sum.y;
+            if (plain)
+                weights(std::false_type{}, shift_m);
+            else
+                weights(std::true_type{}, shift_m);
             tmem_st_wait();
             fence_before();
             bar_arrive(bar(kPFull + tile));
@@ -516,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 if (w.tiles > 0 && ok)
                 {
                     tmem_ld32(o_addr + 32u * c, x);
-                    tmem_ld_wait();
+                    tmem_ld_wait(x);
                 }
                 else
                 {
@@ -524,9 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                     for (int e = 0; e < 32; ++e)
                         x[e] = 0u;
                 }
-                if (!live)
-                    continue;
-                if (w.nsplits > 1)
+                if (live && w.nsplits > 1)
                 {
                     float4 *dst = reinterpret_cast<float4 *>(part + ((uint64_t)w.split * kPromptRows + tid) * D + 32 * c);
 #pragma unroll
@@ -534,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                         dst[e] = make_float4(__uint_as_float(x[4 * e]) * f, __uint_as_float(x[4 * e + 1]) * f,
                                              __uint_as_float(x[4 * e + 2]) * f, __uint_as_float(x[4 * e + 3]) * f);
                 }
-                else
+                else if (live)
                 {
                     uint4 *dst = reinterpret_cast<uint4 *>(out + 32 * c);
 #pragma unroll
@@ -550,15 +624,60 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 }
             }
         }
+        if (w.nsplits > 1)
+        {
+            // ---- the splits are joined by the block that comes last, in their order
+            __threadfence();
+            asm volatile("bar.sync 1, 256;\n" ::: "memory");
+            if (tid == 0)
+                *s_last = atomicAdd(p.counters + item, 1u) == (uint32_t)w.nsplits - 1u;
+            asm volatile("bar.sync 1, 256;\n" ::: "memory");
+            if (*s_last)
+            {
+                __threadfence();
+                if (tid == 0)
+                    p.counters[item] = 0u;
+                uint16_t *rows_out = reinterpret_cast<uint16_t *>(p.out);
+                // a warp per row, a lane per 4 channels
+                for (int r = warp; w.r0 + r < w.r1; r += kSoftWarps)
+                {
+                    const int i = (w.r0 + r) / G, hd = (int)w.h * G + (w.r0 + r) % G;
+                    float top = kKvNegInf, sum = 0.0f;
+                    for (int k = 0; k < w.nsplits; ++k)
+                        top = fmaxf(top, __ldcg(part_lse + k * kPromptRows + r));
+                    const float ref = top == kKvNegInf ? 0.0f : top;
+                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int k = 0; k < w.nsplits; ++k)
+                    {
+                        const float wt = exp2_fast(__ldcg(part_lse + k * kPromptRows + r) - ref);
+                        sum += wt;
+                        if (lane < D / 4)
+                        {
+                            const float4 z = __ldcg(reinterpret_cast<const float4 *>(
+                                part + ((uint64_t)k * kPromptRows + r) * D + 4 * lane));
+                            y.x += wt * z.x, y.y += wt * z.y, y.z += wt * z.z, y.w += wt * z.w;
+                        }
+                    }
+                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    const uint64_t at = (uint64_t)(w.s.row0 + i) * p.heads + hd;
+                    if (lane < D / 4)
+                        *reinterpret_cast<uint2 *>(rows_out + at * D + 4 * lane) =
+                            make_uint2(kv_pack<BF16>(y.x * f, y.y * f), kv_pack<BF16>(y.z * f, y.w * f));
+                    if (lane == 0 && p.lse)
+                        p.lse[at] = (sum == 0.0f ? kKvNegInf : ref + log2f(sum)) * 0.69314718056f;
+                }
+            }
+        }
         fence_before();
     }
     else if (warp < kSoftWarps + kConvWarps)
     {
         // ------------------------------------------------ codes to halves
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kConvRegs));
         constexpr int kPairs = D / 16; // (8 tokens, 16 channels) units of a lane
         const int cw = warp - kSoftWarps;
-        uint4 rk[kPairs], rv[kPairs];
-        int blk[2], nblk[2];  // blocks of the warp's two groups of 16 tokens: loaded tile, next tile
+        uint4 r[kPairs];     // raw bytes of the next half step (a tile's keys, then its values)
+        int blk[2] = {-1, -1}, nblk[2]; // blocks of the warp's two groups of 16 tokens: tile at hand, next tile
         float fk = 0.0f, fv = 0.0f;
         const int bs1 = (1 << shift) - 1;
         auto look = [&](int i, int (&to)[2]) {
@@ -567,38 +686,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             {
                 const int pos = w.base + i * kTok + cw * 32 + u * 16;
                 to[u] = i < w.tiles && pos < w.seen_hi ? kv_block(p.c, w.b, pos >> shift) : -1;
-            }
-        };
-        auto load = [&](int i, const uint8_t *pool, uint64_t stride, uint4 (&r)[kPairs]) {
-#pragma unroll
-            for (int it = 0; it < kPairs; ++it)
-            {
-                const int pair = it * 4 + (lane >> 3), grp = pair / (D / 16), ch = pair % (D / 16);
-                const int tk = grp * 8 + (lane & 7); // token of the warp's 32
-                const int at = grp >= 2 ? blk[1] : blk[0];
-                const int pos = w.base + i * kTok + cw * 32 + tk;
-                r[it] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                if (at >= 0)
-                    r[it] = __ldg(reinterpret_cast<const uint4 *>(
-                        pool + (uint64_t)at * stride + (uint64_t)(((w.h << shift) + (uint32_t)(pos & bs1)) * D + ch * 16)));
-            }
-        };
-        auto convert = [&](uint8_t *tile, const uint4 (&r)[kPairs]) {
-#pragma unroll
-            for (int it = 0; it < kPairs; ++it)
-            {
-                const int pair = it * 4 + (lane >> 3), grp = pair / (D / 16), ch = pair % (D / 16);
-                uint8_t *dst = tile + core_off<D>(cw * 32 + grp * 8 + (lane & 7), 2 * ch);
-                const uint32_t u[4] = {r[it].x, r[it].y, r[it].z, r[it].w};
-                uint32_t y[8];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                {
-                    y[2 * e] = code_halves(u[e], 0x4140);
-                    y[2 * e + 1] = code_halves(u[e], 0x4342);
-                }
-                *reinterpret_cast<uint4 *>(dst) = make_uint4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<uint4 *>(dst + 128) = make_uint4(y[4], y[5], y[6], y[7]);
             }
         };
         auto factors = [&]() { // lane u of the warp: group u
@@ -612,104 +699,153 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             }
         };
         look(0, blk);
-        load(0, p.c.k, p.c.kbs, rk);
-        load(0, p.c.v, p.c.vbs, rv);
         factors();
         look(1, nblk);
-        for (int i = 0; i < w.tiles; ++i)
+        uint32_t live[2] = {0u, 0u}; // values of scale 0 are turned into zeros, whatever their codes
+        // Half step h turns what the one before loaded into halves and loads for the next; one copy of the code, see
+        // the matrix instructions' loop.  Step -1 only loads.
+#pragma unroll 1
+        for (int h = -1; h < 2 * w.tiles; ++h)
         {
-            const int st = i & 1;
-            const uint32_t par = (uint32_t)((i >> 1) + 1) & 1u; // of the stage's release before this use
-            if (i >= 2)
-                ok = bar_wait(bar(kKEmpty + st), par, gave_up);
+            const int i = h >> 1, kind = h & 1, st = i & 1;
+            if (h >= 4)
+                ok = bar_wait(bar(kKEmpty + 2 * kind + st), (uint32_t)((i >> 1) + 1) & 1u, gave_up);
             if (!__all_sync(kKvFull, ok))
                 break;
-            if (lane < 2)
-                s_f[(i % kFactorStages) * kGroups + cw * 2 + lane] =
-                    make_float4(fk, vref > 0.0f ? fv / vref : 0.0f,
-                                __int_as_float((lane ? blk[1] : blk[0]) >= 0 ? w.base + i * kTok + cw * 32 + lane * 16 : kMaxPos), 0.0f);
-            convert(smem + L::k + st * L::kTileBytes, rk);
-            fence_smem();
-            bar_arrive(bar(kKFull + st));
-            blk[0] = nblk[0];
-            blk[1] = nblk[1];
-            load(i + 1, p.c.k, p.c.kbs, rk);
-            factors();
-            if (i >= 2)
-                ok = bar_wait(bar(kVEmpty + st), par, gave_up);
-            if (!__all_sync(kKvFull, ok))
-                break;
-            convert(smem + L::v + st * L::kTileBytes, rv);
-            fence_smem();
-            bar_arrive(bar(kVFull + st));
-            load(i + 1, p.c.v, p.c.vbs, rv);
-            look(i + 2, nblk);
+            if (h >= 0 && kind == 0)
+            {
+                const float rel = fv > 0.0f ? fv / vref : 1.0f; // zeros need no factor
+                const bool held = (lane ? blk[1] : blk[0]) >= 0;
+                if (lane < 2)
+                    s_f[(i % kFactorStages) * kGroups + cw * 2 + lane] =
+                        make_float4(fk, log2f(rel),
+                                    __int_as_float(held ? w.base + i * kTok + cw * 32 + lane * 16 : kMaxPos), 1.0f / rel);
+                live[0] = __shfl_sync(kKvFull, fv, 0) > 0.0f ? kKvFull : 0u;
+                live[1] = __shfl_sync(kKvFull, fv, 1) > 0.0f ? kKvFull : 0u;
+            }
+            const uint32_t keep0 = kind ? live[0] : kKvFull, keep1 = kind ? live[1] : kKvFull;
+            uint8_t *tile = smem + (kind ? L::v : L::k) + st * L::kTileBytes;
+            if (kind && h >= 0)
+            {
+                blk[0] = nblk[0];
+                blk[1] = nblk[1];
+            }
+            if (h >= 0)
+            {
+#pragma unroll
+                for (int it = 0; it < kPairs; ++it)
+                {
+                    const int pair = it * 4 + (lane >> 3), grp = pair / (D / 16), ch = pair % (D / 16);
+                    const int row = cw * 32 + grp * 8 + (lane & 7);
+                    const uint32_t keep = grp >= 2 ? keep1 : keep0, zero = 0x80808080u & ~keep;
+                    const uint32_t u[4] = {(r[it].x & keep) | zero, (r[it].y & keep) | zero, (r[it].z & keep) | zero,
+                                           (r[it].w & keep) | zero};
+                    uint32_t y[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        y[2 * e] = code_halves(u[e], 0x4140);
+                        y[2 * e + 1] = code_halves(u[e], 0x4342);
+                    }
+                    *reinterpret_cast<uint4 *>(tile + tile_off(row, 2 * ch)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint4 *>(tile + tile_off(row, 2 * ch + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+                }
+                fence_smem();
+                bar_arrive(bar(kKFull + 2 * kind + st));
+            }
+            // The loads come behind the fence, which would wait for them.
+            const int in = (h + 1) >> 1; // tile of the next half step
+            const uint8_t *pool = kind ? p.c.k : p.c.v;
+            const uint64_t stride = kind ? p.c.kbs : p.c.vbs;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+            {
+                const int pos = w.base + in * kTok + cw * 32 + u * 16;
+                const uint8_t *src = pool + (uint64_t)max(blk[u], 0) * stride +
+                                     (uint64_t)(((w.h << shift) + (uint32_t)(pos & bs1)) * D) + (lane & 7) * D;
+#pragma unroll
+                for (int it = 0; it < kPairs; ++it)
+                {
+                    const int pair = it * 4 + (lane >> 3), grp = pair / (D / 16), ch = pair % (D / 16);
+                    if (grp >> 1 != u)
+                        continue;
+                    r[it] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                    if (blk[u] >= 0)
+                        r[it] = __ldg(reinterpret_cast<const uint4 *>(src + (grp & 1) * 8 * D + ch * 16));
+                }
+            }
+            if (kind && h >= 0)
+            {
+                factors();
+                look(i + 2, nblk);
+            }
         }
     }
-    else if (lane == 0)
+    else
     {
         // ------------------------------------------------ matrix instructions
-        constexpr uint32_t kRow8 = D / 8 * 128; // from 8 rows to the next
-        constexpr uint32_t kIdS = instr_desc(kTok, false), kIdO = instr_desc(D, true);
-        auto scores = [&](int tile, int st) {
-            const uint32_t a = sbase + L::q + (uint32_t)tile * L::kTileBytes, b = sbase + L::k + (uint32_t)st * L::kTileBytes;
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-                mma_ss(tmem + 128u * (uint32_t)tile, smem_desc(a + 256u * ks, 128u, kRow8),
-                       smem_desc(b + 256u * ks, 128u, kRow8), kIdS, ks > 0 ? 1u : 0u);
-            commit(bar(kSFull + tile));
-        };
-        auto values = [&](int tile, int st, bool first) {
-            const uint32_t b = sbase + L::v + (uint32_t)st * L::kTileBytes;
-#pragma unroll
-            for (int ks = 0; ks < kTok / 16; ++ks)
-                mma_ts(tmem + 256u + (uint32_t)(D * tile), tmem + 128u * (uint32_t)tile + 8u * ks,
-                       smem_desc(b + 2u * kRow8 * ks, kRow8, 128u), kIdO, first && ks == 0 ? 0u : 1u);
-            commit(bar(kODone + tile));
-        };
-        if (w.tiles > 0)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kMmaRegs));
+        if (warp == kMmaWarp)
         {
-            ok = bar_wait(bar(kKFull), 0u, gave_up);
-            fence_after();
-            if (ok)
+            // The whole warp walks the loop and one lane issues: with every address the same in all lanes by
+            // construction (reductions and votes), the operands stay in uniform registers.
+            const uint32_t leader = lane == 0 ? 1u : 0u, tm = __reduce_max_sync(kKvFull, tmem);
+            const uint32_t tiles = __reduce_max_sync(kKvFull, (unsigned)w.tiles);
+            const bool both = __any_sync(kKvFull, two);
+            constexpr uint32_t kIdS = instr_desc(kTok, false), kIdO = instr_desc(D, true);
+            const uint64_t dk = smem_desc(0u, 16u, 1024u), dv = smem_desc(0u, kTok * 128u, 1024u);
+            constexpr uint32_t kNext = L::kTileBytes / 16;
+            const uint32_t aq = (sbase + L::q) >> 4, ak = ((sbase + L::k) >> 4) | (uint32_t)dk;
+            const uint32_t av = ((sbase + L::v) >> 4) | (uint32_t)dv;
+            auto wait = [&](int which, uint32_t parity) {
+                for (uint32_t it = 0; it < kWaitLimit; ++it)
+                {
+                    if (__all_sync(kKvFull, bar_try(bar(which), parity)))
+                        return true;
+                    if ((it & 15u) == 15u && __any_sync(kKvFull, *gave_up != 0))
+                        return false;
+                }
+                *gave_up = 1;
+                return false;
+            };
+            auto scores = [&](uint32_t tile, uint32_t st) {
+                mma_scores<D>(tm + 128u * tile, (aq + tile * kNext) | (uint32_t)dk, ak + st * kNext, (uint32_t)(dk >> 32), kIdS,
+                              leader);
+                commit(bar(kSFull + (int)tile), leader);
+            };
+            const uint32_t ntile = both ? 2u : 1u;
+            // One copy of each piece of this code: between its turns the softmax threads' long loops pass through the
+            // instruction cache.  Turn 0 only starts the scores.
+            bool go = tiles > 0;
+#pragma unroll 1
+            for (uint32_t i = 0; go && i <= tiles; ++i)
             {
-                scores(0, 0);
-                if (two)
-                    scores(1, 0);
-                commit(bar(kKEmpty));
-            }
-        }
-        for (int i = 0; ok && i < w.tiles; ++i)
-        {
-            const int st = i & 1, sn = st ^ 1;
-            const uint32_t par = (uint32_t)(i >> 1) & 1u, parn = (uint32_t)((i + 1) >> 1) & 1u;
-            const bool more = i + 1 < w.tiles;
-            if (!(ok = bar_wait(bar(kVFull + st), par, gave_up)))
-                break;
-            if (!(ok = bar_wait(bar(kPFull), (uint32_t)i & 1u, gave_up)))
-                break;
-            fence_after();
-            values(0, st, i == 0);
-            if (more)
-            {
-                if (!(ok = bar_wait(bar(kKFull + sn), parn, gave_up)))
-                    break;
-                fence_after();
-                scores(0, sn);
-            }
-            if (two)
-            {
-                if (!(ok = bar_wait(bar(kPFull + 1), (uint32_t)i & 1u, gave_up)))
-                    break;
-                fence_after();
-                values(1, st, i == 0);
-            }
-            commit(bar(kVEmpty + st));
-            if (more)
-            {
-                if (two)
-                    scores(1, sn);
-                commit(bar(kKEmpty + sn));
+                const uint32_t sv = (i - 1u) & 1u, sk = i & 1u; // stages of V (tile i - 1) and K (tile i)
+                const bool more = i < tiles;
+                // codes first: the weights' barriers are the ones that come late
+                go = (i == 0 || wait(kVFull + (int)sv, ((i - 1u) >> 1) & 1u)) &&
+                     (!more || wait(kKFull + (int)sk, (i >> 1) & 1u));
+#pragma unroll 1
+                for (uint32_t tile = 0; go && tile < ntile; ++tile)
+                {
+                    if (i > 0)
+                    {
+                        if (!(go = wait(kPFull + (int)tile, sv)))
+                            break;
+                        fence_after();
+                        mma_values(tm + 256u + (uint32_t)D * tile, tm + 128u * tile, av + sv * kNext, (uint32_t)(dv >> 32),
+                                   kIdO, i - 1u, leader);
+                        commit(bar(kODone + (int)tile), leader);
+                    }
+                    else
+                        fence_after();
+                    if (more)
+                        scores(tile, sk);
+                }
+                if (i > 0)
+                    commit(bar(kVEmpty + (int)sv), leader);
+                if (more)
+                    commit(bar(kKEmpty + (int)sk), leader);
             }
         }
     }
@@ -718,66 +854,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
     if (*gave_up)
     {
         // matrix instructions in flight when a wait ran out get a bounded time to end
-        if (tid == 32 * (kSoftWarps + kConvWarps))
+        if (tid == 32 * kMmaWarp)
         {
             atomicAdd(&g_kv_prompt_timeouts, 1u);
-            commit(bar(kDrain));
+            commit(bar(kDrain), 1u);
             for (uint32_t it = 0; it < kWaitLimit && !bar_try(bar(kDrain), 0u); ++it)
             {
             }
         }
         __syncthreads();
     }
-    if (w.nsplits > 1)
-    {
-        // ---- the splits are joined by the block that comes last, in their order
-        const int item = (int)((w.b * p.c.hkv + w.h) * p.row_tiles + rt);
-        const float *part = p.part + (uint64_t)item * p.splits * kPromptRows * (D + 1);
-        const float *part_lse = part + (uint64_t)p.splits * kPromptRows * D;
-        __threadfence();
-        __syncthreads();
-        if (tid == 0)
-            *s_last = atomicAdd(p.counters + item, 1u) == (uint32_t)w.nsplits - 1u;
-        __syncthreads();
-        if (*s_last)
-        {
-            __threadfence();
-            if (tid == 0)
-                p.counters[item] = 0u;
-            uint16_t *out = reinterpret_cast<uint16_t *>(p.out);
-            // a warp per row, a lane per 4 channels
-            for (int r = warp; w.r0 + r < w.r1; r += kThreads / 32)
-            {
-                const int i = (w.r0 + r) / G, hd = (int)w.h * G + (w.r0 + r) % G;
-                float top = kKvNegInf, sum = 0.0f;
-                for (int k = 0; k < w.nsplits; ++k)
-                    top = fmaxf(top, __ldcg(part_lse + k * kPromptRows + r));
-                const float ref = top == kKvNegInf ? 0.0f : top;
-                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int k = 0; k < w.nsplits; ++k)
-                {
-                    const float wt = exp2_fast(__ldcg(part_lse + k * kPromptRows + r) - ref);
-                    sum += wt;
-                    if (lane < D / 4)
-                    {
-                        const float4 z = __ldcg(reinterpret_cast<const float4 *>(
-                            part + ((uint64_t)k * kPromptRows + r) * D + 4 * lane));
-                        y.x += wt * z.x, y.y += wt * z.y, y.z += wt * z.z, y.w += wt * z.w;
-                    }
-                }
-                const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const uint64_t at = (uint64_t)(w.s.row0 + i) * p.heads + hd;
-                if (lane < D / 4)
-                    *reinterpret_cast<uint2 *>(out + at * D + 4 * lane) =
-                        make_uint2(kv_pack<BF16>(y.x * f, y.y * f), kv_pack<BF16>(y.z * f, y.w * f));
-                if (lane == 0 && p.lse)
-                    p.lse[at] = (sum == 0.0f ? kKvNegInf : ref + log2f(sum)) * 0.69314718056f;
-            }
-        }
-    }
     fence_after();
     __syncthreads();
-    if (warp == kSoftWarps + kConvWarps)
+    if (warp == kMmaWarp)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
 }
 
