@@ -20,6 +20,8 @@ struct AttnParams
     float scale_log2;
     const int32_t *blocks; // sparse: rows x hkv x select
     uint32_t select;
+    uint32_t group;     // sparse: query tokens that share a thread block
+    uint32_t groups;    // sparse: such groups of a sequence
     uint32_t chunk;     // cache blocks of one split
     uint32_t splits;    // most splits of a sequence
     uint32_t row_tiles; // row tiles of a (sequence or row, head)
@@ -34,6 +36,7 @@ struct AttnPlan
 {
     bool prompt;  // the kernel of many rows
     uint32_t nt;  // eights of rows of a tile (few rows)
+    uint32_t group, groups; // sparse: see AttnParams
     uint32_t row_tiles, chunk, splits;
     uint64_t blocks_x, bytes;
 };
