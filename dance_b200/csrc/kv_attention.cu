@@ -17,6 +17,8 @@
 // the sum of the weights (taken before rounding) and the output.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "kv_attention.cuh"
 
 namespace dance
@@ -271,56 +273,58 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
     float rf[NT][2];   // logit factor of columns 2t, 2t + 1
     int limit[NT][2];  // tokens that they see
     uint32_t chose[NT][2]; // sparse: their token's bit in the blocks' masks
+    auto load_q = [&]() {
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-    {
-        const int r = r0 + 8 * j + g;
-        float x[D / 4];
-        const bool live = r < r1;
-        const int i = r / G, hd = (int)h * G + r % G;
-        const uint16_t *src = p.q + (uint64_t)(s.row0 + (live ? i : 0)) * p.q_row + (uint64_t)(live ? hd : 0) * p.q_head +
-                              t * (D / 4);
-        if (p.q_aligned)
+        for (int j = 0; j < NT; ++j)
         {
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e)
+            const int r = r0 + 8 * j + g;
+            float x[D / 4];
+            const bool live = r < r1;
+            const int i = r / G, hd = (int)h * G + r % G;
+            const uint16_t *src = p.q + (uint64_t)(s.row0 + (live ? i : 0)) * p.q_row + (uint64_t)(live ? hd : 0) * p.q_head +
+                                  t * (D / 4);
+            if (p.q_aligned)
             {
-                const uint4 w = __ldg(reinterpret_cast<const uint4 *>(src) + e);
-                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    x[8 * e + k] = kv_float<BF16>((uint16_t)(u[k >> 1] >> (16 * (k & 1))));
+                for (int e = 0; e < D / 32; ++e)
+                {
+                    const uint4 w = __ldg(reinterpret_cast<const uint4 *>(src) + e);
+                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        x[8 * e + k] = kv_float<BF16>((uint16_t)(u[k >> 1] >> (16 * (k & 1))));
+                }
             }
-        }
-        else
-        {
+            else
+            {
+#pragma unroll
+                for (int e = 0; e < D / 4; ++e)
+                    x[e] = kv_float<BF16>(src[e]);
+            }
+            float amax = 0.0f;
 #pragma unroll
             for (int e = 0; e < D / 4; ++e)
-                x[e] = kv_float<BF16>(src[e]);
+                amax = fmaxf(amax, fabsf(x[e]));
+            amax = fmaxf(amax, __shfl_xor_sync(kKvFull, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(kKvFull, amax, 2));
+            const int up = row_shift(amax);
+            const float mul = power_of_two(up), back = power_of_two(-up);
+#pragma unroll
+            for (int e = 0; e < 2 * kSteps; ++e)
+                qf[j][e] = live ? kv_pack<false>(x[2 * e] * mul, x[2 * e + 1] * mul) : 0u;
+            const float f = live ? back * p.scale_log2 : 0.0f;
+            rf[j][0] = __shfl_sync(kKvFull, f, (2 * t) << 2);
+            rf[j][1] = __shfl_sync(kKvFull, f, (2 * t + 1) << 2);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+            {
+                const int rr = min(r0 + 8 * j + 2 * t + k, r1 - 1);
+                limit[j][k] = min(s.first + rr / G + 1, s.len);
+                if (SPARSE)
+                    chose[j][k] = 1u << (rr / G - tok_lo);
+            }
         }
-        float amax = 0.0f;
-#pragma unroll
-        for (int e = 0; e < D / 4; ++e)
-            amax = fmaxf(amax, fabsf(x[e]));
-        amax = fmaxf(amax, __shfl_xor_sync(kKvFull, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(kKvFull, amax, 2));
-        const int up = row_shift(amax);
-        const float mul = power_of_two(up), back = power_of_two(-up);
-#pragma unroll
-        for (int e = 0; e < 2 * kSteps; ++e)
-            qf[j][e] = live ? kv_pack<false>(x[2 * e] * mul, x[2 * e + 1] * mul) : 0u;
-        const float f = live ? back * p.scale_log2 : 0.0f;
-        rf[j][0] = __shfl_sync(kKvFull, f, (2 * t) << 2);
-        rf[j][1] = __shfl_sync(kKvFull, f, (2 * t + 1) << 2);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-        {
-            const int rr = min(r0 + 8 * j + 2 * t + k, r1 - 1);
-            limit[j][k] = min(s.first + rr / G + 1, s.len);
-            if (SPARSE)
-                chose[j][k] = 1u << (rr / G - tok_lo);
-        }
-    }
+    };
 
     float o[kSteps][NT][4];
     float m[NT][2], l[NT][2], vref = 0.0f;
@@ -397,7 +401,9 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
 
         for (int st = 0; st < kStages - 1; ++st)
             issue(warp + kWarps * st, st);
-        // the scales, while the first tiles are on their way
+        // q and the scales, while the first tiles are on their way
+        if (seg == e0)
+            load_q();
         for (int e = threadIdx.x; e < padded; e += kWarps * 32)
         {
             const int blk = s_blk[e];
@@ -667,26 +673,40 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
     if (!s_last)
         return;
     __threadfence();
-    float *s_w = reinterpret_cast<float *>(smem); // kRows: 1 / sum, kRows: maximum
-    if (threadIdx.x < kRows)
-    {
-        const int r = threadIdx.x;
-        float top = kKvNegInf, sum = 0.0f;
-        for (int i = 0; i < nsplits; ++i)
-            top = fmaxf(top, __ldcg(part_lse + i * kRows + r));
-        const float base = top == kKvNegInf ? 0.0f : top;
-        for (int i = 0; i < nsplits; ++i)
-            sum += exp2_fast(__ldcg(part_lse + i * kRows + r) - base);
-        s_w[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
-        s_w[kRows + r] = base;
-        if (p.lse && r0 + r < r1)
-        {
-            const int i = (r0 + r) / G, hd = (int)h * G + (r0 + r) % G;
-            p.lse[(uint64_t)(s.row0 + i) * p.heads + hd] = (sum == 0.0f ? kKvNegInf : base + log2f(sum)) * 0.69314718056f;
-        }
-    }
+    float *s_w = reinterpret_cast<float *>(smem); // nsplits x kRows: weights
+    float *s_f = s_w + nsplits * kRows;           // kRows: 1 / sum
+    for (int e = threadIdx.x; e < nsplits * kRows; e += kWarps * 32)
+        s_w[e] = __ldcg(part_lse + e);
+    __syncthreads();
     if (threadIdx.x == 0)
         p.counters[item] = 0u;
+    for (int r = warp; r < kRows; r += kWarps)
+    {
+        float top = kKvNegInf, sum = 0.0f;
+        for (int i = lane; i < nsplits; i += 32)
+            top = fmaxf(top, s_w[i * kRows + r]);
+        for (int o = 16; o; o >>= 1)
+            top = fmaxf(top, __shfl_xor_sync(kKvFull, top, o));
+        const float base = top == kKvNegInf ? 0.0f : top;
+        for (int i = lane; i < nsplits; i += 32)
+        {
+            const float wt = exp2_fast(s_w[i * kRows + r] - base);
+            s_w[i * kRows + r] = wt;
+            sum += wt;
+        }
+        for (int o = 16; o; o >>= 1)
+            sum += __shfl_xor_sync(kKvFull, sum, o);
+        if (lane == 0)
+        {
+            s_f[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
+            if (p.lse && r0 + r < r1)
+            {
+                const int i = (r0 + r) / G, hd = (int)h * G + (r0 + r) % G;
+                p.lse[(uint64_t)(s.row0 + i) * p.heads + hd] =
+                    (sum == 0.0f ? kKvNegInf : base + log2f(sum)) * 0.69314718056f;
+            }
+        }
+    }
     __syncthreads();
     for (int e = threadIdx.x; e < kRows * D / 4; e += kWarps * 32)
     {
@@ -694,13 +714,14 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
         if (r0 + r >= r1)
             break;
         float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
         for (int i = 0; i < nsplits; ++i)
         {
-            const float w = exp2_fast(__ldcg(part_lse + i * kRows + r) - s_w[kRows + r]);
+            const float w = s_w[i * kRows + r];
             const float4 z = __ldcg(reinterpret_cast<const float4 *>(part + ((uint64_t)i * kRows + r) * D + d));
             y.x += w * z.x, y.y += w * z.y, y.z += w * z.z, y.w += w * z.w;
         }
-        const float f = s_w[r];
+        const float f = s_f[r];
         const int i = (r0 + r) / G, hd = (int)h * G + (r0 + r) % G;
         *reinterpret_cast<uint2 *>(out + ((uint64_t)(s.row0 + i) * p.heads + hd) * D + d) =
             make_uint2(kv_pack<BF16>(y.x * f, y.y * f), kv_pack<BF16>(y.z * f, y.w * f));
@@ -708,6 +729,8 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
 }
 
 constexpr uint32_t kSms = 148;
+constexpr uint64_t kMostSplits = 480; // their weights are joined in the ring's shared memory
+static_assert((kMostSplits + 8) * 16 * 4 <= rows_smem<64>(), "weights of the splits");
 constexpr uint64_t kPromptLeast = 32;      // rows of a sequence and key/value head from which it is used
 
 AttnPlan plan_attention(const DanceKvCache &c, const DanceKvBatch &b, uint32_t heads, uint32_t select)
@@ -763,7 +786,8 @@ AttnPlan plan_attention(const DanceKvCache &c, const DanceKvBatch &b, uint32_t h
         // 4 165.  24 of up to 6000, 4 heads: 4 splits 26.7, 7 23.5, 13 33.)
         // Blocks an SM: by shared memory, and by registers for 16 rows.
         const uint32_t per_sm = a.nt == 1 ? (c.head_dim == 128 ? 3u : 4u) : (c.head_dim == 128 ? 2u : 3u);
-        const uint64_t slots = (uint64_t)kSms * per_sm, most = (tokens + 255) / 256;
+        const uint64_t slots = (uint64_t)kSms * per_sm;
+        const uint64_t most = std::min<uint64_t>((tokens + 255) / 256, kMostSplits);
         uint64_t best = ~0ull;
         for (uint64_t waves = 0; waves <= 8; ++waves)
         {

@@ -643,10 +643,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 {
                     const int i = (w.r0 + r) / G, hd = (int)w.h * G + (w.r0 + r) % G;
                     float top = kKvNegInf, sum = 0.0f;
-                    for (int k = 0; k < w.nsplits; ++k)
+                    for (int k = lane; k < w.nsplits; k += 32)
                         top = fmaxf(top, __ldcg(part_lse + k * kPromptRows + r));
+                    for (int o = 16; o; o >>= 1)
+                        top = fmaxf(top, __shfl_xor_sync(kKvFull, top, o));
                     const float ref = top == kKvNegInf ? 0.0f : top;
                     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
                     for (int k = 0; k < w.nsplits; ++k)
                     {
                         const float wt = exp2_fast(__ldcg(part_lse + k * kPromptRows + r) - ref);

@@ -33,6 +33,7 @@ struct SelectParams
     KvView c;
     const uint16_t *q;
     uint64_t q_row, q_head;
+    bool q_aligned;
     uint32_t rows, heads, G;
     uint32_t nblk;      // blocks that a row can see
     uint32_t width;     // floats from one (row, head)'s scores to the next
@@ -126,11 +127,24 @@ __global__ void __launch_bounds__(kScoreThreads) scores_kernel(SelectParams p)
                     const bool live = i < i1;
                     const uint16_t *src = p.q + (uint64_t)(s.row0 + (live ? i : i0)) * p.q_row +
                                           (uint64_t)(h * p.G + g0 + hd) * p.q_head + l8 * (D / 8);
+                    alignas(8) uint16_t raw[D / 8];
+                    if (p.q_aligned) // 8 bytes at a time: D / 8 elements are 16, 24 or 32 bytes
+                    {
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k)
+                            *reinterpret_cast<uint2 *>(&raw[4 * k]) = __ldg(reinterpret_cast<const uint2 *>(src) + k);
+                    }
+                    else
+                    {
+#pragma unroll
+                        for (int k = 0; k < D / 8; ++k)
+                            raw[k] = __ldg(src + k);
+                    }
                     float x[D / 8], amax = 0.0f;
 #pragma unroll
                     for (int k = 0; k < D / 8; ++k)
                     {
-                        x[k] = live ? kv_float<BF16>(__ldg(src + k)) : 0.0f;
+                        x[k] = live ? kv_float<BF16>(raw[k]) : 0.0f;
                         amax = fmaxf(amax, kv_finite_abs(x[k]));
                     }
                     const unsigned eight = 0xFFu << (threadIdx.x & 24);
@@ -375,6 +389,216 @@ __global__ void __launch_bounds__(kChooseThreads) choose_kernel(SelectParams p)
     }
 }
 
+// The same choice for up to 4096 blocks, the keys in registers (KPT of a
+// thread, four adjacent blocks at a time): one read of the scores, and the
+// ranks of all runs from one scan of packed 16-bit counts.
+template <int KPT>
+__global__ void __launch_bounds__(kChooseThreads) choose_short_kernel(SelectParams p)
+{
+    constexpr int kRuns = KPT / 4, kPer = kBins / kChooseThreads;
+    static_assert(kRuns <= 4 && kPer == 8, "16-bit fields of the ranks, two vectors of bins");
+    __shared__ __align__(16) uint32_t hist[kBins];
+    __shared__ uint32_t s_least[kChooseThreads / 32], s_most[kChooseThreads / 32], s_above[kChooseThreads / 32];
+    __shared__ uint32_t s_bin, s_need, s_count;
+    __shared__ __align__(16) uint4 s_ranks[kChooseThreads / 32];
+    const uint32_t b = blockIdx.y, h = blockIdx.x % p.c.hkv;
+    const int i = (int)(blockIdx.x / p.c.hkv), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const KvSeq s = kv_seq(p.c, b, p.rows);
+    if (i >= s.rows)
+        return;
+    const uint64_t rh = (uint64_t)(s.row0 + i) * p.c.hkv + h;
+    int32_t *out = p.out + rh * p.select;
+    const int seen = min(s.first + i + 1, s.len);
+    const int nb = min((max(seen, 0) + (1 << p.c.shift) - 1) >> p.c.shift, (int)p.nblk);
+    const int k = (int)p.select;
+    if (nb <= k)
+    {
+        for (int e = tid; e < k; e += kChooseThreads)
+            out[e] = e < nb ? e : -1;
+        return;
+    }
+    const float4 *sc = reinterpret_cast<const float4 *>(p.scores + rh * p.width);
+    const int lo = (int)p.first, hi = nb - (int)p.last; // the blocks that compete
+    uint32_t need = (uint32_t)(k - (int)p.first - (int)p.last);
+    // Blocks that are always taken get the largest key, places without a block 0: below every score's key, so that
+    // comparisons of keys are all that follows.
+    const int runs = (nb + 4 * kChooseThreads - 1) / (4 * kChooseThreads);
+    uint32_t key[KPT], least = 0xFFFFFFFFu, most = 0u;
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r)
+    {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            key[4 * r + e] = 0u;
+        if (r < runs)
+        {
+            const int q = tid + kChooseThreads * r;
+            const float4 v = 4 * q < nb ? __ldg(sc + q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+                const int j = 4 * q + e;
+                if (j >= lo && j < hi)
+                {
+                    key[4 * r + e] = min(score_key(x[e]), 0xFFFFFFFEu);
+                    least = min(least, key[4 * r + e]);
+                    most = max(most, key[4 * r + e]);
+                }
+                else if (j < nb)
+                    key[4 * r + e] = 0xFFFFFFFFu;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        reinterpret_cast<uint4 *>(hist)[tid * 2 + e] = make_uint4(0u, 0u, 0u, 0u);
+    least = __reduce_min_sync(kKvFull, least);
+    most = __reduce_max_sync(kKvFull, most);
+    if (lane == 0)
+    {
+        s_least[warp] = least;
+        s_most[warp] = most;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kChooseThreads / 32; ++w)
+    {
+        least = min(least, s_least[w]);
+        most = max(most, s_most[w]);
+    }
+    // taken: keys above `top`; of the keys in [least, top] the first `need` in block order
+    uint32_t top = need ? most : 0xFFFFFFFEu;
+    if (!need)
+        least = 0xFFFFFFFEu;
+    while (need)
+    {
+        const uint32_t span = top - least;
+        const int shift = max(0, 21 - __clz(span)); // span >> shift < 2048
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r)
+            if (r < runs)
+            {
+#pragma unroll
+                for (int e = 4 * r; e < 4 * r + 4; ++e)
+                    if (key[e] - least <= span)
+                        atomicAdd(&hist[(key[e] - least) >> shift], 1u);
+            }
+        __syncthreads();
+        // thread t holds eight bins, the highest bins first
+        uint4 *mine = reinterpret_cast<uint4 *>(hist) + (kChooseThreads - 1 - tid) * 2;
+        const uint4 c1 = mine[1], c0 = mine[0];
+        const uint32_t c[kPer] = {c1.w, c1.z, c1.y, c1.x, c0.w, c0.z, c0.y, c0.x};
+        mine[0] = mine[1] = make_uint4(0u, 0u, 0u, 0u);
+        uint32_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+            sum += c[e];
+        uint32_t above = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+        {
+            const uint32_t y = __shfl_up_sync(kKvFull, above, o);
+            above += lane >= o ? y : 0u;
+        }
+        if (lane == 31)
+            s_above[warp] = above;
+        __syncthreads();
+        above -= sum;
+        for (int w = 0; w < warp; ++w)
+            above += s_above[w];
+        if (above < need && above + sum >= need)
+        {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+            {
+                if (above < need && above + c[e] >= need)
+                {
+                    s_bin = (uint32_t)(kBins - 1 - tid * kPer - e);
+                    s_need = need - above;
+                    s_count = c[e];
+                }
+                above += c[e];
+            }
+        }
+        __syncthreads();
+        need = s_need;
+        const uint32_t base = least + (s_bin << shift);
+        top = (uint32_t)min((uint64_t)top, (uint64_t)base + ((1u << shift) - 1u));
+        least = base;
+        if (s_count == need || shift == 0)
+            break;
+    }
+
+    // ranks in block order: run by run, thread by thread; 16 bits for each run
+    const uint32_t span = top - least;
+    uint32_t sure[2] = {0u, 0u}, maybe[2] = {0u, 0u};
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r)
+        if (r < runs)
+        {
+#pragma unroll
+            for (int e = 4 * r; e < 4 * r + 4; ++e)
+            {
+                sure[r >> 1] += key[e] > top ? 1u << (16 * (r & 1)) : 0u;
+                maybe[r >> 1] += key[e] - least <= span ? 1u << (16 * (r & 1)) : 0u;
+            }
+        }
+    uint32_t sure_to[2] = {sure[0], sure[1]}, maybe_to[2] = {maybe[0], maybe[1]};
+    constexpr int kWords = (kRuns + 1) / 2;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+        for (int w = 0; w < kWords; ++w)
+        {
+            const uint32_t y = __shfl_up_sync(kKvFull, sure_to[w], o), z = __shfl_up_sync(kKvFull, maybe_to[w], o);
+            sure_to[w] += lane >= o ? y : 0u;
+            maybe_to[w] += lane >= o ? z : 0u;
+        }
+    if (lane == 31)
+        s_ranks[warp] = make_uint4(sure_to[0], sure_to[1], maybe_to[0], maybe_to[1]);
+    __syncthreads();
+    uint4 all = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int w = 0; w < kWords; ++w)
+    {
+        sure_to[w] -= sure[w];
+        maybe_to[w] -= maybe[w];
+    }
+#pragma unroll
+    for (int w = 0; w < kChooseThreads / 32; ++w)
+    {
+        const uint4 y = s_ranks[w];
+        if (w < warp)
+        {
+            sure_to[0] += y.x, sure_to[1] += y.y;
+            maybe_to[0] += y.z, maybe_to[1] += y.w;
+        }
+        all.x += y.x, all.y += y.y, all.z += y.z, all.w += y.w;
+    }
+    uint32_t sure_base = 0, maybe_base = 0;
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r)
+        if (r < runs)
+        {
+            const int sh = 16 * (r & 1);
+            uint32_t a = sure_base + ((sure_to[r >> 1] >> sh) & 0xFFFFu);
+            uint32_t m = maybe_base + ((maybe_to[r >> 1] >> sh) & 0xFFFFu);
+#pragma unroll
+            for (int e = 4 * r; e < 4 * r + 4; ++e)
+            {
+                const int j = 4 * (tid + kChooseThreads * r) + (e & 3);
+                const bool in = key[e] - least <= span;
+                if (key[e] > top || (in && m < need))
+                    out[min(a + min(m, need), (uint32_t)k - 1u)] = j;
+                a += key[e] > top;
+                m += in;
+            }
+            sure_base += ((r >> 1 ? all.y : all.x) >> sh) & 0xFFFFu;
+            maybe_base += ((r >> 1 ? all.w : all.z) >> sh) & 0xFFFFu;
+        }
+}
+
 uint32_t score_blocks(const DanceKvCache &c, const DanceKvBatch &b)
 {
     const uint64_t n = ((uint64_t)b.max_len + c.block_tokens - 1) / c.block_tokens;
@@ -416,7 +640,13 @@ int launch_select(SelectParams &p, bool bf16, cudaStream_t st)
         if (int rc = p.c.max_rows <= 8 ? launch_scores<D, 1>(p, bf16, st) : launch_scores<D, 4>(p, bf16, st))
             return rc;
     const dim3 grid(p.c.max_rows * p.c.hkv, p.c.batch);
-    if (p.nblk <= kChooseKeys)
+    if (p.nblk <= 4 * kChooseThreads)
+        choose_short_kernel<4><<<grid, kChooseThreads, 0, st>>>(p);
+    else if (p.nblk <= 8 * kChooseThreads)
+        choose_short_kernel<8><<<grid, kChooseThreads, 0, st>>>(p);
+    else if (p.nblk <= 16 * kChooseThreads)
+        choose_short_kernel<16><<<grid, kChooseThreads, 0, st>>>(p);
+    else if (p.nblk <= kChooseKeys)
         choose_kernel<true><<<grid, kChooseThreads, p.nblk * 4, st>>>(p);
     else
         choose_kernel<false><<<grid, kChooseThreads, 0, st>>>(p);
@@ -464,6 +694,7 @@ extern "C" int dance_kv_select_blocks(const DanceKvCache *cache, const DanceKvBa
     p.q = reinterpret_cast<const uint16_t *>(q->d_data);
     p.q_row = q->row_stride;
     p.q_head = q->head_stride;
+    p.q_aligned = kv_aligned(*q);
     p.rows = q->rows;
     p.heads = num_heads;
     p.G = num_heads / cache->kv_heads;

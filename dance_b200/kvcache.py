@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from ctypes import addressof as _address
 
 from . import DANCE_BF16, DANCE_F16, DANCE_F32, DanceKvBatch, DanceKvCache, DanceKvRows, check, load
 
@@ -83,6 +84,8 @@ class KVCache:
         self._c = DanceKvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), bounds.data_ptr(),
                                max(k.stride(0), least), max(v.stride(0), least), n, h, bs, d)
         self._ptr = ctypes.addressof(self._c)
+        self._index = k.get_device()
+        self._key = (n, h, bs, d, self._index)
 
     @classmethod
     def create(cls, num_blocks: int, kv_heads: int, head_dim: int, block_tokens: int = 64, device="cuda"):
@@ -127,6 +130,8 @@ class KVBatch:
         self._c = DanceKvBatch(block_table.data_ptr(), seq_lens.data_ptr(), row_offsets.data_ptr(),
                                block_table.shape[1], n, self.max_rows, self.max_len)
         self._ptr = ctypes.addressof(self._c)
+        self._index = seq_lens.get_device()
+        self._key = (n, self.max_rows, self.max_len, block_table.shape[1])
 
 
 class KVWorkspace:
@@ -137,66 +142,70 @@ class KVWorkspace:
         self._t = None
         self._ptr = 0
         self._bytes = 0
-        self._known = {}
+        self._known = set()
 
     def reserve(self, cache: KVCache, batch: KVBatch, rows: int, num_heads: int, select: int = 0) -> None:
         """Room for such a call (before a stream capture, which must not allocate)."""
-        key = (cache._c.num_blocks, cache.kv_heads, cache.block_tokens, cache.head_dim, batch.batch, batch.max_rows,
-               batch.max_len, batch._c.table_width, rows, num_heads, select, cache.device.index)
-        need = self._known.get(key)
-        if need is None:
+        key = (cache._key, batch._key, rows, num_heads, select)
+        if key not in self._known:
             need = load().dance_kv_workspace_bytes(cache._ptr, batch._ptr, rows, num_heads, select)
             if need == 0:
                 check(-1, "dance_kv_workspace_bytes")
+            if need > self._bytes or self._t.device != cache.device:
+                import torch
+                self._t = torch.zeros(need, dtype=torch.uint8, device=cache.device)
+                self._ptr, self._bytes = self._t.data_ptr(), need
+                self._known.clear()  # what it held room for may have been on another device
             if len(self._known) > 256:
                 self._known.clear()
-            self._known[key] = need
-        if need > self._bytes or self._t.device != cache.device:
-            import torch
-            self._t = torch.zeros(need, dtype=torch.uint8, device=cache.device)
-            self._ptr, self._bytes = self._t.data_ptr(), need
+            self._known.add(key)
 
 
+# The calls below are short (a decode step calls them once per layer), so what
+# they need of torch is bound once, on the first call.
+_torch = None
+_lib = None
 _DTYPES: dict = {}
 
 
-def _codes():
-    if not _DTYPES:
-        import torch
-        _DTYPES.update({torch.float16: DANCE_F16, torch.bfloat16: DANCE_BF16, torch.float32: DANCE_F32})
-    return _DTYPES
+def _bind():
+    global _torch, _lib
+    import torch
+    _lib = load()
+    _DTYPES.update({torch.float16: DANCE_F16, torch.bfloat16: DANCE_BF16, torch.float32: DANCE_F32})
+    _torch = torch
 
 
 def _rows(name, x, cache, heads=None):
     """DanceKvRows of a (rows, heads, head_dim) tensor."""
-    import torch
-    if not isinstance(x, torch.Tensor) or x.dim() != 3 or not x.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor of three dimensions")
-    code = _codes().get(x.dtype)
+    try:
+        n, h, d = x.shape
+        s0, s1, s2 = x.stride()
+        code = _DTYPES.get(x.dtype)
+        index = x.get_device()
+    except (AttributeError, TypeError, ValueError):
+        raise ValueError(f"{name} must be a CUDA tensor of three dimensions") from None
     if code is None or code == DANCE_F32:
         raise TypeError(f"{name} is {x.dtype}: float16 or bfloat16 is needed")
-    n, h, d = x.shape
-    s = x.stride()
-    if d != cache.head_dim or (heads is not None and h != heads) or (heads is None and (h == 0 or h % cache.kv_heads)):
+    if d != cache.head_dim or (h != heads if heads is not None else h == 0 or h % cache.kv_heads):
         raise ValueError(f"{name} has shape {tuple(x.shape)}: the cache has {cache.kv_heads} heads of {cache.head_dim}")
-    if s[2] != 1:
+    if s2 != 1:
         raise ValueError(f"{name}: the channels must be contiguous")
-    if x.device != cache.device:
+    if index != cache._index:
         raise ValueError(f"{name} lies on {x.device}, the cache on {cache.device}")
-    return DanceKvRows(x.data_ptr(), s[0], s[1], n, code)
+    return DanceKvRows(x.data_ptr(), s0, s1, n, code), n, h
 
 
-def _same_device(cache, batch):
-    if batch.device != cache.device:
+def _enter(cache, batch):
+    """Checks the devices; torch's current stream, on which outputs and scratch are allocated too."""
+    if _torch is None:
+        _bind()
+    index = cache._index
+    if batch._index != index:
         raise ValueError(f"the batch lies on {batch.device}, the cache on {cache.device}")
-
-
-def _current(device):
-    """torch's current stream, on which outputs and scratch are allocated too."""
-    import torch
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"the cache lies on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    if _torch._C._cuda_getDevice() != index:
+        raise ValueError(f"the cache lies on {cache.device}, the current device is cuda:{_torch.cuda.current_device()}")
+    return _torch._C._cuda_getCurrentRawStream(index)
 
 
 def _streamed(fn):
@@ -219,12 +228,12 @@ def append(cache: KVCache, batch: KVBatch, k, v) -> None:
     the cache.  The scales of touched blocks only grow; where one does, the
     block's earlier codes are rounded again.  NaN becomes 0, an infinity the
     largest code."""
-    _same_device(cache, batch)
-    kr, vr = _rows("k", k, cache, cache.kv_heads), _rows("v", v, cache, cache.kv_heads)
-    if kr.rows != vr.rows or kr.dtype != vr.dtype:
+    stream = _enter(cache, batch)
+    kr, n, _ = _rows("k", k, cache, cache.kv_heads)
+    vr, m, _ = _rows("v", v, cache, cache.kv_heads)
+    if n != m or k.dtype != v.dtype:
         raise ValueError(f"k is {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}")
-    rc = load().dance_kv_append(cache._ptr, batch._ptr, ctypes.addressof(kr), ctypes.addressof(vr),
-                                _current(cache.device))
+    rc = _lib.dance_kv_append(cache._ptr, batch._ptr, _address(kr), _address(vr), stream)
     if rc:
         check(rc, "dance_kv_append")
 
@@ -234,58 +243,56 @@ def read(cache: KVCache, batch: KVBatch, rows: int, dtype=None):
     """(keys, values) that the cache holds for the batch's rows, each (rows,
     kv_heads, head_dim) of dtype (float16, bfloat16 or float32; None: float16).
     The keys of a head are a vector store that an index build takes."""
-    import torch
-    _same_device(cache, batch)
-    dtype = dtype or torch.float16
-    code = _codes().get(dtype)
+    stream = _enter(cache, batch)
+    dtype = dtype or _torch.float16
+    code = _DTYPES.get(dtype)
     if code is None:
         raise TypeError(f"dtype {dtype}: float16, bfloat16 or float32 is needed")
     if rows < 0:
         raise ValueError("rows must not be negative")
-    k = torch.empty((rows, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
-    v = torch.empty_like(k)
-    rc = load().dance_kv_read(cache._ptr, batch._ptr, rows, code, k.data_ptr(), v.data_ptr(),
-                              _current(cache.device))
+    both = _torch.empty((2, rows, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
+    k, v = both.unbind(0)
+    rc = _lib.dance_kv_read(cache._ptr, batch._ptr, rows, code, k.data_ptr(), v.data_ptr(), stream)
     if rc:
         check(rc, "dance_kv_read")
     return k, v
 
 
 def _attend(cache, batch, q, blocks, scale, return_lse, out, workspace):
-    import torch
-    _same_device(cache, batch)
-    qr = _rows("q", q, cache)
-    rows, heads, dim = q.shape
-    st = _current(cache.device)
+    stream = _enter(cache, batch)
+    qr, rows, heads = _rows("q", q, cache)
+    dim = cache.head_dim
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=cache.device)
+        out = _torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     else:
         _cuda("out", out, q.dtype, q.shape)
         _need(out.is_contiguous() and out.device == cache.device, "out must be contiguous, on the cache's device")
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=cache.device) if return_lse else None
-    select = 0
+    lse, lse_ptr, select = None, None, 0
+    if return_lse:
+        lse = _torch.empty((rows, heads), dtype=_torch.float32, device=cache.device)
+        lse_ptr = lse.data_ptr()
     if blocks is not None:
-        if blocks.dim() != 3 or blocks.shape[0] != rows or blocks.shape[1] != cache.kv_heads or not blocks.is_cuda:
+        if blocks.dim() != 3 or blocks.shape[0] != rows or blocks.shape[1] != cache.kv_heads:
             raise ValueError(f"blocks has shape {tuple(blocks.shape)}: ({rows}, {cache.kv_heads}, select) is needed")
-        if blocks.dtype != torch.int32:
+        if blocks.dtype != _torch.int32:
             raise TypeError(f"blocks is {blocks.dtype}, torch.int32 is needed")
         select = blocks.shape[2]
-        _need(blocks.is_contiguous() and blocks.device == cache.device, "blocks must be contiguous, on the cache's device")
-        _need(1 <= select <= 4096, f"{select} blocks per row: 1 to 4096 are supported")
+        if not blocks.is_contiguous() or blocks.get_device() != cache._index:
+            raise ValueError("blocks must be contiguous, on the cache's device")
+        if not 1 <= select <= 4096:
+            raise ValueError(f"{select} blocks per row: 1 to 4096 are supported")
     ws = workspace or KVWorkspace()
     ws.reserve(cache, batch, rows, heads, select)
     if scale is None:
         scale = dim ** -0.5
-    lse_ptr = lse.data_ptr() if return_lse else None
-    lib = load()
     if blocks is None:
-        rc = lib.dance_kv_attention(cache._ptr, batch._ptr, ctypes.addressof(qr), heads, scale, out.data_ptr(),
-                                    lse_ptr, ws._ptr, ws._bytes, st)
+        rc = _lib.dance_kv_attention(cache._ptr, batch._ptr, _address(qr), heads, scale, out.data_ptr(), lse_ptr,
+                                     ws._ptr, ws._bytes, stream)
         if rc:
             check(rc, "dance_kv_attention")
     else:
-        rc = lib.dance_kv_sparse_attention(cache._ptr, batch._ptr, ctypes.addressof(qr), heads, blocks.data_ptr(),
-                                           select, scale, out.data_ptr(), lse_ptr, ws._ptr, ws._bytes, st)
+        rc = _lib.dance_kv_sparse_attention(cache._ptr, batch._ptr, _address(qr), heads, blocks.data_ptr(), select,
+                                            scale, out.data_ptr(), lse_ptr, ws._ptr, ws._bytes, stream)
         if rc:
             check(rc, "dance_kv_sparse_attention")
     return (out, lse) if return_lse else out
@@ -319,22 +326,19 @@ def select_blocks(cache: KVCache, batch: KVBatch, q, select: int, *, first_block
     (rows, kv_heads, select), ascending, -1 filled.  The row's first
     ``first_blocks`` and last ``last_blocks`` blocks are always among them, the
     others have the largest upper bounds on their logits."""
-    import torch
-    _same_device(cache, batch)
-    qr = _rows("q", q, cache)
-    rows, heads, _ = q.shape
+    stream = _enter(cache, batch)
+    qr, rows, heads = _rows("q", q, cache)
     if not 1 <= select <= 4096 or first_blocks < 0 or last_blocks < 0 or first_blocks + last_blocks > select:
         raise ValueError(f"select {select} (1 to 4096) must hold {first_blocks} first and {last_blocks} last blocks")
-    st = _current(cache.device)
     if out is None:
-        out = torch.empty((rows, cache.kv_heads, select), dtype=torch.int32, device=cache.device)
+        out = _torch.empty((rows, cache.kv_heads, select), dtype=_torch.int32, device=cache.device)
     else:
-        _cuda("out", out, torch.int32, (rows, cache.kv_heads, select))
+        _cuda("out", out, _torch.int32, (rows, cache.kv_heads, select))
         _need(out.is_contiguous() and out.device == cache.device, "out must be contiguous, on the cache's device")
     ws = workspace or KVWorkspace()
     ws.reserve(cache, batch, rows, heads, select)
-    rc = load().dance_kv_select_blocks(cache._ptr, batch._ptr, ctypes.addressof(qr), heads, select, first_blocks,
-                                       last_blocks, out.data_ptr(), ws._ptr, ws._bytes, st)
+    rc = _lib.dance_kv_select_blocks(cache._ptr, batch._ptr, _address(qr), heads, select, first_blocks, last_blocks,
+                                     out.data_ptr(), ws._ptr, ws._bytes, stream)
     if rc:
         check(rc, "dance_kv_select_blocks")
     return out
