@@ -1,9 +1,9 @@
 // kv_cache.cu -- the write into and the read out of the 8-bit key/value cache
 // (dance_kv_append, dance_kv_read in include/dance_b200.h).
 //
-// append.  One thread block per (touched cache block, head, keys or values).
-// Its new rows are read once into registers; their largest finite magnitude
-// and the scale so far give the new scale.  Only where that grew are the
+// append.  One thread block per (touched cache block, head), keys and values.
+// The new rows are read once into registers; their largest finite
+// magnitudes and the scales so far give the new scales.  Only where that grew are the
 // block's earlier codes read, rounded again and written back.  The earlier
 // tokens enter the bounds through the bounds themselves (rounding is monotone,
 // so the rounded bounds are the bounds of the rounded codes), so that a decode
@@ -32,22 +32,74 @@ struct AppendParams
     bool aligned[2];
 };
 
-// The largest of a non-negative value over the thread block.
-__device__ __forceinline__ float block_max(float x, float *s)
+// Two magnitudes at once, as the bits of two 16-bit floats without their sign:
+// such bits order like the values, infinities and NaN above all.
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// The largest finite magnitude of eight values.
+template <bool BF16>
+__device__ __noinline__ float finite_max(uint4 x)
+{
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    float m = 0.0f;
+    for (int e = 0; e < 4; ++e)
+    {
+        m = fmaxf(m, kv_finite_abs(kv_float<BF16>((uint16_t)w[e])));
+        m = fmaxf(m, kv_finite_abs(kv_float<BF16>((uint16_t)(w[e] >> 16))));
+    }
+    return m;
+}
+
+// Four finite values at a scale as codes.  Adding 1.5 * 2^23 + 128 rounds to a
+// whole number, ties to even as rint does (the sum's unit is 1 and the number
+// added is even), and leaves the code in the low byte; |x * inv| is at most
+// 127 up to rounding, so nothing is cut off.
+template <bool BF16>
+__device__ __forceinline__ uint32_t codes4(uint32_t w0, uint32_t w1, float inv)
+{
+    const float magic = 12582912.0f + 128.0f;
+    const uint32_t a = __float_as_uint(__fadd_rn(__fmul_rn(kv_float<BF16>((uint16_t)w0), inv), magic));
+    const uint32_t b = __float_as_uint(__fadd_rn(__fmul_rn(kv_float<BF16>((uint16_t)(w0 >> 16)), inv), magic));
+    const uint32_t c = __float_as_uint(__fadd_rn(__fmul_rn(kv_float<BF16>((uint16_t)w1), inv), magic));
+    const uint32_t d = __float_as_uint(__fadd_rn(__fmul_rn(kv_float<BF16>((uint16_t)(w1 >> 16)), inv), magic));
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// The same for any values; not inlined, so that it costs the common case a
+// branch and no more.
+template <bool BF16>
+__device__ __noinline__ uint32_t codes4_any(uint32_t w0, uint32_t w1, float inv)
+{
+    uint32_t r = 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        r |= (uint32_t)(kv_code(kv_float<BF16>((uint16_t)((e < 2 ? w0 : w1) >> (16 * (e & 1)))), inv) + 128) << (8 * e);
+    return r;
+}
+
+// The largest of two non-negative values over the thread block.
+__device__ __forceinline__ float2 block_max(float2 x, float2 *s)
 {
     for (int o = 16; o; o >>= 1)
-        x = fmaxf(x, __shfl_xor_sync(kKvFull, x, o));
+    {
+        x.x = fmaxf(x.x, __shfl_xor_sync(kKvFull, x.x, o));
+        x.y = fmaxf(x.y, __shfl_xor_sync(kKvFull, x.y, o));
+    }
     if ((threadIdx.x & 31) == 0)
         s[threadIdx.x >> 5] = x;
     __syncthreads();
-    float m = 0.0f;
+    float2 m = make_float2(0.0f, 0.0f);
     for (int i = 0; i < (int)blockDim.x / 32; ++i)
-        m = fmaxf(m, s[i]);
+        m = make_float2(fmaxf(m.x, s[i].x), fmaxf(m.y, s[i].y));
     return m;
 }
 
 // Four codes rounded again to a scale that is 1 / shrink times as large.
-__device__ __forceinline__ uint32_t shrink_codes(uint32_t w, float shrink)
+__device__ __noinline__ uint32_t shrink_codes(uint32_t w, float shrink)
 {
     uint32_t r = 0u;
 #pragma unroll
@@ -61,15 +113,16 @@ __device__ __forceinline__ uint32_t shrink_codes(uint32_t w, float shrink)
 
 // IT = block_tokens / 16 tokens per thread.
 template <int D, int IT, bool BF16>
-__global__ void __launch_bounds__(D / 8 * kTokenGroups) append_kernel(AppendParams p)
+__global__ void __launch_bounds__(D / 8 * kTokenGroups, IT <= 2 ? 1536 / (D / 8 * kTokenGroups) : 1)
+    append_kernel(AppendParams p)
 {
     constexpr int kD8 = D / 8, kBs = IT * kTokenGroups;
-    __shared__ float red[8];
+    __shared__ float2 red[8];
     __shared__ uint2 lo_s[kTokenGroups][kD8], hi_s[kTokenGroups][kD8];
-    const uint32_t b = blockIdx.z, h = blockIdx.y >> 1, kind = blockIdx.y & 1u;
+    const uint32_t b = blockIdx.y, h = blockIdx.x % p.c.hkv; // heads of a token side by side
     const KvSeq s = kv_seq(p.c, b, p.rows);
     const int start = max(s.first, 0), end = s.first + s.rows;
-    const int page = start / kBs + (int)blockIdx.x;
+    const int page = start / kBs + (int)(blockIdx.x / p.c.hkv);
     const int base = page * kBs;
     const int lo = max(start, base), hi = min(end, base + kBs);
     if (lo >= hi)
@@ -80,110 +133,138 @@ __global__ void __launch_bounds__(D / 8 * kTokenGroups) append_kernel(AppendPara
     const int n_old = lo - base;
     const int d8 = threadIdx.x % kD8, tg = threadIdx.x / kD8;
     const uint64_t si = (uint64_t)blk * p.c.hkv + h;
-    uint8_t *codes = (kind ? p.c.v + (uint64_t)blk * p.c.vbs : p.c.k + (uint64_t)blk * p.c.kbs) +
-                     (uint64_t)h * (kBs * D) + d8 * 8;
-    float *scales = kind ? p.c.vs : p.c.ks;
-    const uint16_t *x0 = p.x[kind] + (uint64_t)h * p.head_stride[kind] + d8 * 8;
-    const float old = n_old ? scales[si] : 0.0f;
+    const float old[2] = {n_old ? p.c.ks[si] : 0.0f, n_old ? p.c.vs[si] : 0.0f};
 
-    uint4 x[IT];
-    float amax = 0.0f;
+    uint4 x[2][IT];
 #pragma unroll
-    for (int i = 0; i < IT; ++i)
-    {
-        const int pos = base + tg + kTokenGroups * i;
-        x[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (pos >= lo && pos < hi)
+    for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
         {
-            const uint16_t *src = x0 + (uint64_t)(s.row0 + pos - s.first) * p.row_stride[kind];
-            if (p.aligned[kind])
-                x[i] = __ldg(reinterpret_cast<const uint4 *>(src));
-            else
+            const int pos = base + tg + kTokenGroups * i;
+            x[kind][i] = make_uint4(0u, 0u, 0u, 0u);
+            if (pos >= lo && pos < hi)
             {
-                uint32_t w[4];
+                const uint16_t *src = p.x[kind] + (uint64_t)h * p.head_stride[kind] + d8 * 8 +
+                                      (uint64_t)(s.row0 + pos - s.first) * p.row_stride[kind];
+                if (p.aligned[kind])
+                    x[kind][i] = __ldg(reinterpret_cast<const uint4 *>(src));
+                else
+                {
+                    uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    w[e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
-                x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
+                    x[kind][i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
             }
         }
-    }
+    float amax[2];
+    bool odd = false; // infinities or NaN among the thread's values
 #pragma unroll
-    for (int i = 0; i < IT; ++i)
+    for (int kind = 0; kind < 2; ++kind)
     {
-        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t top = 0u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int i = 0; i < IT; ++i)
         {
-            amax = fmaxf(amax, kv_finite_abs(kv_float<BF16>((uint16_t)w[e])));
-            amax = fmaxf(amax, kv_finite_abs(kv_float<BF16>((uint16_t)(w[e] >> 16))));
+            top = max_u16x2(top, max_u16x2(x[kind][i].x & 0x7FFF7FFFu, x[kind][i].y & 0x7FFF7FFFu));
+            top = max_u16x2(top, max_u16x2(x[kind][i].z & 0x7FFF7FFFu, x[kind][i].w & 0x7FFF7FFFu));
+        }
+        const uint32_t most = max(top & 0xFFFFu, top >> 16);
+        amax[kind] = kv_float<BF16>((uint16_t)most);
+        odd |= most >= (BF16 ? 0x7F80u : 0x7C00u);
+    }
+    if (odd)
+    {
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind)
+        {
+            amax[kind] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+                amax[kind] = fmaxf(amax[kind], finite_max<BF16>(x[kind][i]));
         }
     }
-    amax = block_max(amax, red);
-    const float scale = fmaxf(old, kv_scale_of(amax));
-    const float inv = kv_inverse(scale);
-    // a scale that was never written (NaN) cannot be told from a grown one: the comparison treats it as grown
-    const bool grew = n_old > 0 && !(scale == old);
-    const float shrink = scale > 0.0f ? __fdiv_rn(old, scale) : 0.0f;
+    const float2 both = block_max(make_float2(amax[0], amax[1]), red);
 
     uint32_t lo4[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, hi4[2] = {0u, 0u};
+    float key_shrink = 1.0f;
+    bool key_grew = false;
 #pragma unroll
-    for (int i = 0; i < IT; ++i)
+    for (int kind = 0; kind < 2; ++kind)
     {
-        const int t = tg + kTokenGroups * i, pos = base + t;
-        if (pos >= lo && pos < hi)
+        const float scale = fmaxf(old[kind], kv_scale_of(kind ? both.y : both.x));
+        const float inv = kv_inverse(scale);
+        // a scale that was never written (NaN) cannot be told from a grown one: the comparison treats it as grown
+        const bool grew = n_old > 0 && !(scale == old[kind]);
+        const float shrink = scale > 0.0f ? __fdiv_rn(old[kind], scale) : 0.0f;
+        uint8_t *codes = (kind ? p.c.v + (uint64_t)blk * p.c.vbs : p.c.k + (uint64_t)blk * p.c.kbs) +
+                         (uint64_t)h * (kBs * D) + d8 * 8;
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
         {
-            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            uint32_t q[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
+            const int t = tg + kTokenGroups * i, pos = base + t;
+            if (pos >= lo && pos < hi)
             {
-                q[2 * e] = (uint32_t)(kv_code(kv_float<BF16>((uint16_t)w[e]), inv) + 128);
-                q[2 * e + 1] = (uint32_t)(kv_code(kv_float<BF16>((uint16_t)(w[e] >> 16)), inv) + 128);
+                const uint4 w = x[kind][i];
+                uint32_t c2[2];
+                if (odd)
+                {
+                    c2[0] = codes4_any<BF16>(w.x, w.y, inv);
+                    c2[1] = codes4_any<BF16>(w.z, w.w, inv);
+                }
+                else
+                {
+                    c2[0] = codes4<BF16>(w.x, w.y, inv);
+                    c2[1] = codes4<BF16>(w.z, w.w, inv);
+                }
+                *reinterpret_cast<uint2 *>(codes + t * D) = make_uint2(c2[0], c2[1]);
+                if (kind == 0)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+                    {
+                        lo4[g] = __vminu4(lo4[g], c2[g]);
+                        hi4[g] = __vmaxu4(hi4[g], c2[g]);
+                    }
             }
-            const uint32_t c2[2] = {q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24),
-                                    q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24)};
-            *reinterpret_cast<uint2 *>(codes + t * D) = make_uint2(c2[0], c2[1]);
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
+            else if (grew && t < n_old)
             {
-                lo4[g] = __vminu4(lo4[g], c2[g]);
-                hi4[g] = __vmaxu4(hi4[g], c2[g]);
+                const uint2 c = *reinterpret_cast<const uint2 *>(codes + t * D);
+                *reinterpret_cast<uint2 *>(codes + t * D) =
+                    make_uint2(shrink_codes(c.x, shrink), shrink_codes(c.y, shrink));
             }
         }
-        else if (grew && t < n_old)
+        if (threadIdx.x == 0)
+            (kind ? p.c.vs : p.c.ks)[si] = scale;
+        if (kind == 0)
         {
-            const uint2 c = *reinterpret_cast<const uint2 *>(codes + t * D);
-            *reinterpret_cast<uint2 *>(codes + t * D) = make_uint2(shrink_codes(c.x, shrink), shrink_codes(c.y, shrink));
+            key_shrink = shrink;
+            key_grew = grew;
         }
     }
-    if (threadIdx.x == 0)
-        scales[si] = scale;
-    if (kind == 0)
+    lo_s[tg][d8] = make_uint2(lo4[0], lo4[1]);
+    hi_s[tg][d8] = make_uint2(hi4[0], hi4[1]);
+    __syncthreads();
+    if (threadIdx.x < 2 * kD8)
     {
-        lo_s[tg][d8] = make_uint2(lo4[0], lo4[1]);
-        hi_s[tg][d8] = make_uint2(hi4[0], hi4[1]);
-        __syncthreads();
-        if (threadIdx.x < 2 * kD8)
+        const bool high = threadIdx.x >= kD8;
+        const int d = high ? threadIdx.x - kD8 : threadIdx.x;
+        uint2 *out = reinterpret_cast<uint2 *>(p.c.bounds + (2 * si + (high ? 1 : 0)) * D) + d;
+        uint2 r = high ? make_uint2(0u, 0u) : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
+        if (n_old)
         {
-            const bool high = threadIdx.x >= kD8;
-            const int d = high ? threadIdx.x - kD8 : threadIdx.x;
-            uint2 *out = reinterpret_cast<uint2 *>(p.c.bounds + (2 * si + (high ? 1 : 0)) * D) + d;
-            uint2 r = high ? make_uint2(0u, 0u) : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
-            if (n_old)
-            {
-                r = *out;
-                if (grew)
-                    r = make_uint2(shrink_codes(r.x, shrink), shrink_codes(r.y, shrink));
-            }
-            for (int g = 0; g < kTokenGroups; ++g)
-            {
-                const uint2 y = high ? hi_s[g][d] : lo_s[g][d];
-                r.x = high ? __vmaxu4(r.x, y.x) : __vminu4(r.x, y.x);
-                r.y = high ? __vmaxu4(r.y, y.y) : __vminu4(r.y, y.y);
-            }
-            *out = r;
+            r = *out;
+            if (key_grew)
+                r = make_uint2(shrink_codes(r.x, key_shrink), shrink_codes(r.y, key_shrink));
         }
+        for (int g = 0; g < kTokenGroups; ++g)
+        {
+            const uint2 y = high ? hi_s[g][d] : lo_s[g][d];
+            r.x = high ? __vmaxu4(r.x, y.x) : __vminu4(r.x, y.x);
+            r.y = high ? __vmaxu4(r.y, y.y) : __vminu4(r.y, y.y);
+        }
+        *out = r;
     }
 }
 
@@ -246,7 +327,11 @@ __global__ void __launch_bounds__(256) read_kernel(KvView c, uint32_t rows, void
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                y[k] = __fmul_rn((float)((int)(((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 255u) - 128), scale);
+            {
+                // the byte as the last of 2^23 + c, exactly
+                const uint32_t u = __byte_perm(k < 4 ? w.x : w.y, 0x4B000000u, 0x7440 + (k & 3));
+                y[k] = __fmul_rn(__fsub_rn(__uint_as_float(u), 8388608.0f + 128.0f), scale);
+            }
             if constexpr (DT == DANCE_F32)
             {
                 float4 *o = reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + out);
@@ -310,7 +395,7 @@ extern "C" int dance_kv_append(const DanceKvCache *cache, const DanceKvBatch *ba
     }
     p.rows = k->rows;
     const uint32_t bs = cache->block_tokens;
-    const dim3 grid((batch->max_rows + bs - 2) / bs + 1, 2 * cache->kv_heads, batch->batch);
+    const dim3 grid(((batch->max_rows + bs - 2) / bs + 1) * cache->kv_heads, batch->batch);
     const bool bf16 = k->dtype == DANCE_BF16;
     switch (cache->head_dim)
     {
