@@ -62,8 +62,8 @@ constexpr int kGroups = kTok / 16;    // 16 tokens share a cache block
 constexpr int kFactorStages = 4;      // factors are read up to two tiles after the codes are free
 constexpr float kLift = 7.0f;         // log2 of the weight of a row's reference maximum
 constexpr float kSlack = 8.0f;        // how far the maximum may rise above the reference
-constexpr uint32_t kWaitNs = 20000;       // how long one try may sleep
-constexpr uint32_t kWaitLimit = 1u << 16; // tries
+constexpr uint32_t kWaitNs = 20000;           // how long one try may sleep
+constexpr long long kWaitClocks = 2000000000; // about a second: a wait in earnest is over in microseconds
 
 template <int D>
 struct Layout
@@ -116,13 +116,10 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 {
     if (bar_try(bar, parity))
         return true;
-    for (uint32_t it = 0; it < kWaitLimit; ++it)
-    {
+    const long long begin = clock64();
+    while (clock64() - begin < kWaitClocks && !*gave_up)
         if (bar_try(bar, parity))
             return true;
-        if ((it & 15u) == 15u && *gave_up)
-            return false;
-    }
     *gave_up = 1;
     return false;
 }
@@ -801,13 +798,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             const uint32_t aq = (sbase + L::q) >> 4, ak = ((sbase + L::k) >> 4) | (uint32_t)dk;
             const uint32_t av = ((sbase + L::v) >> 4) | (uint32_t)dv;
             auto wait = [&](int which, uint32_t parity) {
-                for (uint32_t it = 0; it < kWaitLimit; ++it)
-                {
+                if (__all_sync(kKvFull, bar_try(bar(which), parity)))
+                    return true;
+                const long long begin = clock64();
+                while (__all_sync(kKvFull, clock64() - begin < kWaitClocks && !*gave_up))
                     if (__all_sync(kKvFull, bar_try(bar(which), parity)))
                         return true;
-                    if ((it & 15u) == 15u && __any_sync(kKvFull, *gave_up != 0))
-                        return false;
-                }
                 *gave_up = 1;
                 return false;
             };
@@ -861,7 +857,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         {
             atomicAdd(&g_kv_prompt_timeouts, 1u);
             commit(bar(kDrain), 1u);
-            for (uint32_t it = 0; it < kWaitLimit && !bar_try(bar(kDrain), 0u); ++it)
+            const long long begin = clock64();
+            while (!bar_try(bar(kDrain), 0u) && clock64() - begin < kWaitClocks)
             {
             }
         }

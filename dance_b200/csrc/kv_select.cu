@@ -10,6 +10,12 @@
 // of an integer sum does not show, so the choice is the same however it is
 // summed.
 //
+// Floor: the bounds' 2 * head_dim bytes of every (block, head), once.  Measured:
+// 32 sequences of up to 1875 blocks, 8 heads of 128 channels (54.7 MB): 28 us,
+// scores 19 (2.9 TB/s), choice 6, a launch between them.  700 rows of one
+// sequence, 24 heads of 96, 2049 blocks: 94 us, scores 46, choice 47; both
+// kernels wait on latency there, not on the 4 us that bytes and products need.
+//
 // scores_kernel writes the float scores of (row, head, block) from integer
 // matrix instructions, choose_kernel finds each (row, head)'s threshold in
 // histograms of the order-preserving keys and writes the chosen blocks in
@@ -68,8 +74,13 @@ constexpr int code_stride()
 // maximum over the query heads stays in the accumulator's lane.  A warp keeps
 // the bounds of its 32 blocks in registers through all heads and rows; a lane
 // takes adjacent bytes, the order of the channels in the sum being free.
+//
+// Latency bounds it (prologue, then bounds loaded in their turn), so blocks an
+// SM count most: 700 rows x 24 heads x 2049 blocks of 96 channels took 61 us
+// with 32 rows a block and no register bound, 53 with four blocks an SM, 46
+// with 16 rows and four, 50 with five (spills); 8 and 64 rows were slower.
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(kScoreThreads) scores_kernel(SelectParams p)
+__global__ void __launch_bounds__(kScoreThreads, 4) scores_kernel(SelectParams p)
 {
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int kRows = 8 * NT, kStride = code_stride<D>(), kChunks = 2 * D / 64;
@@ -637,7 +648,7 @@ template <int D>
 int launch_select(SelectParams &p, bool bf16, cudaStream_t st)
 {
     if (p.nblk > p.select)
-        if (int rc = p.c.max_rows <= 8 ? launch_scores<D, 1>(p, bf16, st) : launch_scores<D, 4>(p, bf16, st))
+        if (int rc = p.c.max_rows <= 8 ? launch_scores<D, 1>(p, bf16, st) : launch_scores<D, 2>(p, bf16, st))
             return rc;
     const dim3 grid(p.c.max_rows * p.c.hkv, p.c.batch);
     if (p.nblk <= 4 * kChooseThreads)
@@ -685,6 +696,10 @@ extern "C" int dance_kv_select_blocks(const DanceKvCache *cache, const DanceKvBa
         return 0;
     if (!d_blocks || (uintptr_t)d_blocks % 4)
         return fail(-1, "null or misaligned output");
+    if ((uint64_t)batch->max_rows * cache->kv_heads > 0x7FFFFFFFull ||
+        (uint64_t)(batch->max_rows / 8 + 1) * (score_blocks(*cache, *batch) / kScoreBlocks + 1) > 0x7FFFFFFFull)
+        return fail(-1, "call too large: max_rows %u, %u heads, %u blocks", batch->max_rows, cache->kv_heads,
+                    score_blocks(*cache, *batch));
     const uint64_t need = kv_counter_bytes() + kv_select_bytes(*cache, *batch, q->rows);
     if (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < need)
         return fail(-1, "workspace of %llu bytes: %llu are needed", (unsigned long long)workspace_bytes,
