@@ -298,77 +298,57 @@ int launch_append(const AppendParams &p, dim3 grid, bool bf16, cudaStream_t st)
     return 0;
 }
 
-constexpr int kReadRows = 16;
-
-// Eight codes at a scale, stored as DT.
-template <int DT>
-__device__ __forceinline__ void store8(void *dst, uint64_t at, uint32_t w0, uint32_t w1, float scale)
-{
-    float y[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-    {
-        // the byte as the last of 2^23 + c, exactly
-        const uint32_t u = __byte_perm(k < 4 ? w0 : w1, 0x4B000000u, 0x7440 + (k & 3));
-        y[k] = __fmul_rn(__fsub_rn(__uint_as_float(u), 8388608.0f + 128.0f), scale);
-    }
-    if constexpr (DT == DANCE_F32)
-    {
-        float4 *o = reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + at);
-        o[0] = make_float4(y[0], y[1], y[2], y[3]);
-        o[1] = make_float4(y[4], y[5], y[6], y[7]);
-    }
-    else
-    {
-        constexpr bool bf = DT == DANCE_BF16;
-        *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(dst) + at) = make_uint4(
-            kv_pack<bf>(y[0], y[1]), kv_pack<bf>(y[2], y[3]), kv_pack<bf>(y[4], y[5]), kv_pack<bf>(y[6], y[7]));
-    }
-}
-
-// A thread block takes 16 rows, a thread 16 channels of a (row, head) at a
-// time, keys and values: two 16-byte loads in flight for each.
+// One thread per 8 channels of a (row, head): 8 code bytes in, 8 values out.
 template <int D, int DT>
 __global__ void __launch_bounds__(256) read_kernel(KvView c, uint32_t rows, void *ko, void *vo)
 {
-    constexpr uint32_t kD16 = D / 16;
-    const uint32_t b = blockIdx.y, per_row = c.hkv * kD16, mask = (1u << c.shift) - 1u;
+    constexpr uint32_t kD8 = D / 8;
+    const uint32_t b = blockIdx.y;
     const KvSeq s = kv_seq(c, b, rows);
-    for (int64_t r0 = (int64_t)blockIdx.x * kReadRows; r0 < s.rows; r0 += (int64_t)gridDim.x * kReadRows)
+    const uint64_t n = (uint64_t)s.rows * c.hkv * kD8;
+    const uint32_t mask = (1u << c.shift) - 1u;
+    for (uint64_t e = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (uint64_t)gridDim.x * blockDim.x)
     {
-        const uint32_t units = (uint32_t)min((int64_t)kReadRows, s.rows - r0) * per_row;
-#pragma unroll 3
-        for (uint32_t e = threadIdx.x; e < units; e += 256)
-        {
-            const uint32_t dr = e / per_row, x = e - dr * per_row, h = x / kD16, d = (x - h * kD16) * 16;
-            const int i = (int)r0 + (int)dr, pos = s.first + i;
-            const int blk = pos >= 0 ? kv_block(c, b, pos >> c.shift) : -1;
-            const uint64_t si = (uint64_t)max(blk, 0) * c.hkv + h;
-            const uint64_t in = (uint64_t)(((h << c.shift) + ((uint32_t)pos & mask)) * D + d);
-            const uint64_t out = ((uint64_t)(s.row0 + i) * c.hkv + h) * D + d;
-            uint4 w[2];
-            float scale[2];
+        const uint32_t d8 = (uint32_t)(e % kD8), rh = (uint32_t)(e / kD8), h = rh % c.hkv, i = rh / c.hkv;
+        const int pos = s.first + (int)i;
+        const int blk = pos >= 0 ? kv_block(c, b, pos >> c.shift) : -1;
+        const uint64_t si = (uint64_t)max(blk, 0) * c.hkv + h;
+        const uint64_t in = (((uint64_t)h << c.shift) + ((uint32_t)pos & mask)) * D + d8 * 8;
+        const uint64_t out = ((uint64_t)(s.row0 + i) * c.hkv + h) * D + d8 * 8;
 #pragma unroll
-            for (int kind = 0; kind < 2; ++kind)
+        for (int kind = 0; kind < 2; ++kind)
+        {
+            void *dst = kind ? vo : ko;
+            if (!dst)
+                continue;
+            float y[8];
+            uint2 w = make_uint2(0x80808080u, 0x80808080u);
+            float scale = 0.0f;
+            if (blk >= 0)
             {
-                w[kind] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                scale[kind] = 0.0f;
-                if (blk >= 0 && (kind ? vo : ko))
-                {
-                    w[kind] = __ldg(reinterpret_cast<const uint4 *>(
-                        (kind ? c.v + (uint64_t)blk * c.vbs : c.k + (uint64_t)blk * c.kbs) + in));
-                    scale[kind] = __ldg((kind ? c.vs : c.ks) + si);
-                }
+                w = __ldg(reinterpret_cast<const uint2 *>(
+                    (kind ? c.v + (uint64_t)blk * c.vbs : c.k + (uint64_t)blk * c.kbs) + in));
+                scale = __ldg((kind ? c.vs : c.ks) + si);
             }
 #pragma unroll
-            for (int kind = 0; kind < 2; ++kind)
+            for (int k = 0; k < 8; ++k)
             {
-                void *dst = kind ? vo : ko;
-                if (dst)
-                {
-                    store8<DT>(dst, out, w[kind].x, w[kind].y, scale[kind]);
-                    store8<DT>(dst, out + 8, w[kind].z, w[kind].w, scale[kind]);
-                }
+                // the byte as the last of 2^23 + c, exactly
+                const uint32_t u = __byte_perm(k < 4 ? w.x : w.y, 0x4B000000u, 0x7440 + (k & 3));
+                y[k] = __fmul_rn(__fsub_rn(__uint_as_float(u), 8388608.0f + 128.0f), scale);
+            }
+            if constexpr (DT == DANCE_F32)
+            {
+                float4 *o = reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + out);
+                o[0] = make_float4(y[0], y[1], y[2], y[3]);
+                o[1] = make_float4(y[4], y[5], y[6], y[7]);
+            }
+            else
+            {
+                constexpr bool bf = DT == DANCE_BF16;
+                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(dst) + out) =
+                    make_uint4(kv_pack<bf>(y[0], y[1]), kv_pack<bf>(y[2], y[3]), kv_pack<bf>(y[4], y[5]),
+                               kv_pack<bf>(y[6], y[7]));
             }
         }
     }
@@ -377,7 +357,8 @@ __global__ void __launch_bounds__(256) read_kernel(KvView c, uint32_t rows, void
 template <int D>
 int launch_read(const KvView &c, uint32_t rows, int dtype, void *ko, void *vo, cudaStream_t st)
 {
-    const dim3 grid((c.max_rows + kReadRows - 1) / kReadRows, c.batch);
+    const uint64_t work = (uint64_t)c.max_rows * c.hkv * (D / 8);
+    const dim3 grid((unsigned)((work + 255) / 256 < 65536 ? (work + 255) / 256 : 65536), c.batch);
     if (dtype == DANCE_F32)
         read_kernel<D, DANCE_F32><<<grid, 256, 0, st>>>(c, rows, ko, vo);
     else if (dtype == DANCE_F16)
