@@ -5,24 +5,29 @@
 // two tiles of 128, one tensor-memory lane per row, and walks the sequence in
 // tiles of 128 tokens:
 //   S = Q K^T   (A, B in shared memory, f16, sums in tensor memory)
-//   P = weights (softmax threads: S from tensor memory, P back over it as f16)
+//   P = weights (softmax threads: S from tensor memory, P back to it as f16)
 //   O += P V    (A = P from tensor memory, B in shared memory)
-// The two row tiles alternate, so that the tensor core works on one while the
-// softmax threads work on the other.  Tensor memory is full: 2 x 128 columns
-// of S (P lies over the first half of its S) and 2 x head_dim of O.
+// The two row tiles alternate.  A row's 128 logits move into registers at
+// once, so one S serves both tiles: the scores of the other tile, and then of
+// the next token tile, are computed while the weights are.  Tensor memory: 128
+// columns of S, 2 x 64 of P, 2 x head_dim of O, full at 128 channels.
 //
 // Measured on 2594 rows x 32 heads over 16000 and 7100 tokens of 128 channels:
-// 0.82 ms, 0.69 PFLOP/s (0.41 of the measured matrix rate).  What bounds it is
-// the chain softmax -> P V -> Q K^T of each row tile, about 5300 clocks for
-// 128 tokens where the tensor core works 2100: tensor core, exponentials and
-// issue slots are each under half used.  Tried and slower, from 0.88 to 0.90
-// ms: scores in two buffers of 64 columns computed ahead, 0.94 (a product of
-// 64 columns takes the tensor core as long as one of 128); weights handed over
-// in halves, 0.95; a quarter of the exponentials as polynomials, 0.95.  What
-// helped: the row's logits read from tensor memory once, 1.21 -> 0.88 together
-// with registers handed to the softmax threads; one short copy of the code
-// that issues the products (it competes with long unrolled loops for the
-// instruction cache), 0.90 -> 0.86.
+// 0.78 ms, 0.72 PFLOP/s (0.43 of the measured matrix rate).  A token tile takes
+// about 4900 clocks where the tensor core works 2100: what bounds it are the
+// softmax threads' 3200 clocks for a tile (two warps a scheduler, the
+// exponentials half of it) and the turning of codes into halves; tensor core,
+// exponentials and issue slots are each under half used.  Tried and slower:
+// an S for each row tile with P over it, so that softmax and both products of a
+// tile follow one another, 0.82; with two buffers of 64 columns each, 0.94 (a
+// product of 64 columns takes the tensor core as long as one of 128); weights
+// handed over in halves, 0.95; a quarter of the exponentials as polynomials,
+// 0.95; one register buffer of raw codes instead of two, 0.84; 176 registers
+// for the softmax threads, 0.86, which then spill.  What helped before: the
+// logits read from tensor memory once, 1.21 -> 0.88 together with registers
+// handed to the softmax threads; one short copy of the code that issues the
+// products (it competes with long unrolled loops for the instruction cache),
+// 0.90 -> 0.86.
 //
 // Warps 0-3 and 4-7 hold the rows' softmax, one thread per row and no exchange
 // between threads.  Warps 8-11 turn codes into halves: a tile's raw bytes are
@@ -54,9 +59,9 @@ namespace
 constexpr int kSoftWarps = 8, kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps;
 // Four groups of four warps, so that registers can be handed between them (the
-// last group's other warps only wait): 128 x (2 x 192 + 80 + 48) = 512 x 128.
+// last group's other warps only wait): 128 x (2 x 184 + 96 + 48) = 512 x 128.
 constexpr int kThreads = 512;
-constexpr int kSoftRegs = 192, kConvRegs = 80, kMmaRegs = 48;
+constexpr int kSoftRegs = 184, kConvRegs = 96, kMmaRegs = 48;
 constexpr int kTok = (int)kPromptTokens;
 constexpr int kGroups = kTok / 16;    // 16 tokens share a cache block
 constexpr int kFactorStages = 4;      // factors are read up to two tiles after the codes are free
@@ -90,7 +95,8 @@ enum Bar : int
     kSFull = 8,  // 2 row tiles
     kPFull = 10,
     kODone = 12,
-    kDrain = 14
+    kSFree = 14,
+    kDrain = 15
 };
 
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count)
@@ -344,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             bar_init(bar(kPFull + i), 128);
             bar_init(bar(kODone + i), 1);
         }
+        bar_init(bar(kSFree), 128);
         bar_init(bar(kDrain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         *gave_up = 0;
@@ -423,14 +430,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftRegs));
         const int tile = warp >> 2;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21; // tensor-memory lane in bits 16 and up
-        const uint32_t s_addr = tmem + lanes + 128u * (uint32_t)tile;
+        const uint32_t s_addr = tmem + lanes, p_addr = s_addr + 128u + 64u * (uint32_t)tile;
         const uint32_t o_addr = tmem + lanes + 256u + (uint32_t)(D * tile);
         const int tile_lo = min(w.s.first + (w.r0 + 128 * tile) / G + 1, w.s.len); // least that a row of the tile sees
         for (int i = 0; i < (tile == 0 || two ? w.tiles : 0); ++i)
         {
-            // the product before these scores is done as well (the tensor core works in order)
-            ok = bar_wait(bar(kSFull + tile), (uint32_t)i & 1u, gave_up) &&
-                 (i == 0 || bar_wait(bar(kODone + tile), (uint32_t)(i - 1) & 1u, gave_up));
+            ok = bar_wait(bar(kSFull + tile), (uint32_t)i & 1u, gave_up);
             if (!__all_sync(kKvFull, ok))
             {
                 ok = false;
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                         }
                         l = fmaf(sum.x + sum.y, fg.w, l);
                     }
-                    tmem_st16(s_addr + 16u * c, y);
+                    tmem_st16(p_addr + 16u * c, y);
                 }
             };
             if (whole)
@@ -519,10 +524,23 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 maximum(std::true_type{}, 0);
             tmem_ld_wait(x[2]);
             loaded(x[3]);
+            fence_before();
+            bar_arrive(bar(kSFree)); // the other row tile's scores may take its place
             if (whole)
                 maximum(std::false_type{}, kGroups / 2);
             else
                 maximum(std::true_type{}, kGroups / 2);
+            // the product before is done with O and with the place of the weights
+            if (i > 0)
+            {
+                ok = bar_wait(bar(kODone + tile), (uint32_t)(i - 1) & 1u, gave_up);
+                if (!__all_sync(kKvFull, ok))
+                {
+                    ok = false;
+                    break;
+                }
+                fence_after();
+            }
             const bool rise = top > m + kSlack; // from -inf: any maximum
             if (__any_sync(kKvFull, rise))
             {
@@ -676,8 +694,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kConvRegs));
         constexpr int kPairs = D / 16; // (8 tokens, 16 channels) units of a lane
         const int cw = warp - kSoftWarps;
-        uint4 r[kPairs];     // raw bytes of the next half step (a tile's keys, then its values)
-        int blk[2] = {-1, -1}, nblk[2]; // blocks of the warp's two groups of 16 tokens: tile at hand, next tile
+        uint4 rk[kPairs], rv[kPairs];          // raw bytes, loaded a tile ahead
+        int blk[2] = {-1, -1}, nblk[2]; // blocks of the warp's two groups of 16 tokens: loaded tile, next tile
         float fk = 0.0f, fv = 0.0f;
         const int bs1 = (1 << shift) - 1;
         auto look = [&](int i, int (&to)[2]) {
@@ -688,79 +706,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 to[u] = i < w.tiles && pos < w.seen_hi ? kv_block(p.c, w.b, pos >> shift) : -1;
             }
         };
-        auto factors = [&]() { // lane u of the warp: group u
-            fk = fv = 0.0f;
-            const int mine = lane ? blk[1] : blk[0];
-            if (lane < 2 && mine >= 0)
-            {
-                const uint64_t si = (uint64_t)mine * p.c.hkv + w.h;
-                fk = __ldg(p.c.ks + si);
-                fv = __ldg(p.c.vs + si);
-            }
-        };
-        look(0, blk);
-        factors();
-        look(1, nblk);
-        uint32_t live[2] = {0u, 0u}; // values of scale 0 are turned into zeros, whatever their codes
-        // Half step h turns what the one before loaded into halves and loads for the next; one copy of the code, see
-        // the matrix instructions' loop.  Step -1 only loads.
-#pragma unroll 1
-        for (int h = -1; h < 2 * w.tiles; ++h)
-        {
-            const int i = h >> 1, kind = h & 1, st = i & 1;
-            if (h >= 4)
-                ok = bar_wait(bar(kKEmpty + 2 * kind + st), (uint32_t)((i >> 1) + 1) & 1u, gave_up);
-            if (!__all_sync(kKvFull, ok))
-                break;
-            if (h >= 0 && kind == 0)
-            {
-                const float rel = fv > 0.0f ? fv / vref : 1.0f; // zeros need no factor
-                const bool held = (lane ? blk[1] : blk[0]) >= 0;
-                if (lane < 2)
-                    s_f[(i % kFactorStages) * kGroups + cw * 2 + lane] =
-                        make_float4(fk, log2f(rel),
-                                    __int_as_float(held ? w.base + i * kTok + cw * 32 + lane * 16 : kMaxPos), 1.0f / rel);
-                live[0] = __shfl_sync(kKvFull, fv, 0) > 0.0f ? kKvFull : 0u;
-                live[1] = __shfl_sync(kKvFull, fv, 1) > 0.0f ? kKvFull : 0u;
-            }
-            const uint32_t keep0 = kind ? live[0] : kKvFull, keep1 = kind ? live[1] : kKvFull;
-            uint8_t *tile = smem + (kind ? L::v : L::k) + st * L::kTileBytes;
-            if (kind && h >= 0)
-            {
-                blk[0] = nblk[0];
-                blk[1] = nblk[1];
-            }
-            if (h >= 0)
-            {
-#pragma unroll
-                for (int it = 0; it < kPairs; ++it)
-                {
-                    const int pair = it * 4 + (lane >> 3), grp = pair / (D / 16), ch = pair % (D / 16);
-                    const int row = cw * 32 + grp * 8 + (lane & 7);
-                    const uint32_t keep = grp >= 2 ? keep1 : keep0, zero = 0x80808080u & ~keep;
-                    const uint32_t u[4] = {(r[it].x & keep) | zero, (r[it].y & keep) | zero, (r[it].z & keep) | zero,
-                                           (r[it].w & keep) | zero};
-                    uint32_t y[8];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                    {
-                        y[2 * e] = code_halves(u[e], 0x4140);
-                        y[2 * e + 1] = code_halves(u[e], 0x4342);
-                    }
-                    *reinterpret_cast<uint4 *>(tile + tile_off(row, 2 * ch)) = make_uint4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<uint4 *>(tile + tile_off(row, 2 * ch + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
-                }
-                fence_smem();
-                bar_arrive(bar(kKFull + 2 * kind + st));
-            }
-            // The loads come behind the fence, which would wait for them.
-            const int in = (h + 1) >> 1; // tile of the next half step
-            const uint8_t *pool = kind ? p.c.k : p.c.v;
-            const uint64_t stride = kind ? p.c.kbs : p.c.vbs;
+        auto load = [&](int i, const uint8_t *pool, uint64_t stride, uint4 (&r)[kPairs]) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
             {
-                const int pos = w.base + in * kTok + cw * 32 + u * 16;
+                const int pos = w.base + i * kTok + cw * 32 + u * 16;
                 const uint8_t *src = pool + (uint64_t)max(blk[u], 0) * stride +
                                      (uint64_t)(((w.h << shift) + (uint32_t)(pos & bs1)) * D) + (lane & 7) * D;
 #pragma unroll
@@ -774,11 +724,76 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                         r[it] = __ldg(reinterpret_cast<const uint4 *>(src + (grp & 1) * 8 * D + ch * 16));
                 }
             }
-            if (kind && h >= 0)
+        };
+        auto convert = [&](uint8_t *tile, const uint4 (&r)[kPairs], uint32_t keep0, uint32_t keep1) {
+#pragma unroll
+            for (int it = 0; it < kPairs; ++it)
             {
-                factors();
-                look(i + 2, nblk);
+                const int pair = it * 4 + (lane >> 3), grp = pair / (D / 16), ch = pair % (D / 16);
+                const int row = cw * 32 + grp * 8 + (lane & 7);
+                const uint32_t keep = grp >= 2 ? keep1 : keep0, zero = 0x80808080u & ~keep;
+                const uint32_t u[4] = {(r[it].x & keep) | zero, (r[it].y & keep) | zero, (r[it].z & keep) | zero,
+                                       (r[it].w & keep) | zero};
+                uint32_t y[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    y[2 * e] = code_halves(u[e], 0x4140);
+                    y[2 * e + 1] = code_halves(u[e], 0x4342);
+                }
+                *reinterpret_cast<uint4 *>(tile + tile_off(row, 2 * ch)) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4 *>(tile + tile_off(row, 2 * ch + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
             }
+        };
+        auto factors = [&]() { // lane u of the warp: group u
+            fk = fv = 0.0f;
+            const int mine = lane ? blk[1] : blk[0];
+            if (lane < 2 && mine >= 0)
+            {
+                const uint64_t si = (uint64_t)mine * p.c.hkv + w.h;
+                fk = __ldg(p.c.ks + si);
+                fv = __ldg(p.c.vs + si);
+            }
+        };
+        look(0, blk);
+        load(0, p.c.k, p.c.kbs, rk);
+        load(0, p.c.v, p.c.vbs, rv);
+        factors();
+        look(1, nblk);
+#pragma unroll 1
+        for (int i = 0; i < w.tiles; ++i)
+        {
+            const int st = i & 1;
+            const uint32_t par = (uint32_t)((i >> 1) + 1) & 1u; // of the stage's release before this use
+            if (i >= 2)
+                ok = bar_wait(bar(kKEmpty + st), par, gave_up);
+            if (!__all_sync(kKvFull, ok))
+                break;
+            const float rel = fv > 0.0f ? fv / vref : 1.0f; // values of scale 0 become zeros and need no factor
+            const bool held = (lane ? blk[1] : blk[0]) >= 0;
+            if (lane < 2)
+                s_f[(i % kFactorStages) * kGroups + cw * 2 + lane] =
+                    make_float4(fk, log2f(rel),
+                                __int_as_float(held ? w.base + i * kTok + cw * 32 + lane * 16 : kMaxPos), 1.0f / rel);
+            const uint32_t live[2] = {__shfl_sync(kKvFull, fv, 0) > 0.0f ? kKvFull : 0u,
+                                      __shfl_sync(kKvFull, fv, 1) > 0.0f ? kKvFull : 0u};
+            convert(smem + L::k + st * L::kTileBytes, rk, kKvFull, kKvFull);
+            fence_smem();
+            bar_arrive(bar(kKFull + st));
+            if (i >= 2)
+                ok = bar_wait(bar(kVEmpty + st), par, gave_up);
+            if (!__all_sync(kKvFull, ok))
+                break;
+            convert(smem + L::v + st * L::kTileBytes, rv, live[0], live[1]);
+            fence_smem();
+            bar_arrive(bar(kVFull + st));
+            // the next tile's loads come behind the fences, which would wait for them
+            blk[0] = nblk[0];
+            blk[1] = nblk[1];
+            load(i + 1, p.c.k, p.c.kbs, rk);
+            load(i + 1, p.c.v, p.c.vbs, rv);
+            factors();
+            look(i + 2, nblk);
         }
     }
     else
@@ -807,44 +822,41 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 *gave_up = 1;
                 return false;
             };
-            auto scores = [&](uint32_t tile, uint32_t st) {
-                mma_scores<D>(tm + 128u * tile, (aq + tile * kNext) | (uint32_t)dk, ak + st * kNext, (uint32_t)(dk >> 32), kIdS,
-                              leader);
-                commit(bar(kSFull + (int)tile), leader);
-            };
             const uint32_t ntile = both ? 2u : 1u;
             // One copy of each piece of this code: between its turns the softmax threads' long loops pass through the
-            // instruction cache.  Turn 0 only starts the scores.
-            bool go = tiles > 0;
+            // instruction cache.  Step n issues the scores of row tile n % ntile over token tile n / ntile, as soon as
+            // the scores before have been read, and then the product with V of ntile steps before.
+            const uint32_t steps = tiles * ntile;
 #pragma unroll 1
-            for (uint32_t i = 0; go && i <= tiles; ++i)
+            for (uint32_t n = 0; n < steps + ntile; ++n)
             {
-                const uint32_t sv = (i - 1u) & 1u, sk = i & 1u; // stages of V (tile i - 1) and K (tile i)
-                const bool more = i < tiles;
-                // codes first: the weights' barriers are the ones that come late
-                go = (i == 0 || wait(kVFull + (int)sv, ((i - 1u) >> 1) & 1u)) &&
-                     (!more || wait(kKFull + (int)sk, (i >> 1) & 1u));
-#pragma unroll 1
-                for (uint32_t tile = 0; go && tile < ntile; ++tile)
+                const uint32_t tile = both ? n & 1u : 0u, i = both ? n >> 1 : n; // scores' token tile
+                const uint32_t sk = i & 1u, sv = sk ^ 1u;
+                if (n < steps)
                 {
-                    if (i > 0)
-                    {
-                        if (!(go = wait(kPFull + (int)tile, sv)))
-                            break;
-                        fence_after();
-                        mma_values(tm + 256u + (uint32_t)D * tile, tm + 128u * tile, av + sv * kNext, (uint32_t)(dv >> 32),
-                                   kIdO, i - 1u, leader);
-                        commit(bar(kODone + (int)tile), leader);
-                    }
-                    else
-                        fence_after();
-                    if (more)
-                        scores(tile, sk);
+                    if (tile == 0 && !wait(kKFull + (int)sk, (i >> 1) & 1u))
+                        break;
+                    if (n > 0 && !wait(kSFree, (n - 1u) & 1u))
+                        break;
+                    fence_after();
+                    mma_scores<D>(tm, (aq + tile * kNext) | (uint32_t)dk, ak + sk * kNext, (uint32_t)(dk >> 32), kIdS, leader);
+                    commit(bar(kSFull + (int)tile), leader);
+                    if (tile + 1 == ntile)
+                        commit(bar(kKEmpty + (int)sk), leader);
                 }
-                if (i > 0)
-                    commit(bar(kVEmpty + (int)sv), leader);
-                if (more)
-                    commit(bar(kKEmpty + (int)sk), leader);
+                if (n >= ntile)
+                {
+                    if (tile == 0 && !wait(kVFull + (int)sv, ((i - 1u) >> 1) & 1u))
+                        break;
+                    if (!wait(kPFull + (int)tile, sv))
+                        break;
+                    fence_after();
+                    mma_values(tm + 256u + (uint32_t)D * tile, tm + 128u + 64u * tile, av + sv * kNext, (uint32_t)(dv >> 32),
+                               kIdO, i - 1u, leader);
+                    commit(bar(kODone + (int)tile), leader);
+                    if (tile + 1 == ntile)
+                        commit(bar(kVEmpty + (int)sv), leader);
+                }
             }
         }
     }
