@@ -237,7 +237,7 @@ def _append(s):
         x = torch.where(fresh[..., None, None], x, 0.0).permute(0, 1, 3, 2, 4)[used]
         f, o = fresh[used][:, None, :, None], older[used][:, None, :, None]
         size = torch.where(x.isfinite(), x.abs(), 0.0).amax((2, 3))
-        new = size / torch.full_like(size, 127.0)  # by a number torch multiplies with its reciprocal
+        new = size / 127.0
         new = torch.where(new < TINY, 0.0, new)
         old = torch.where(o.any(2)[:, :, 0], s[name + "_scale"][blk_ids], 0.0)
         scale = torch.maximum(old, new)
@@ -298,8 +298,7 @@ def _select(s):
     G, R, q = case["heads"] // hkv, s["max_rows"], s["q"].float()
     off = s["offsets"].long()
     B, W = s["table"].shape
-    size = torch.where(q.isfinite(), q.abs(), 0.0).amax(-1, keepdim=True)
-    size = size / torch.full_like(size, 127.0)
+    size = torch.where(q.isfinite(), q.abs(), 0.0).amax(-1, keepdim=True) / 127.0
     size = torch.where(size < TINY, 0.0, size)
     c = _quantised(q, size).view(-1, hkv, G, dim)
     table = s["table"].clamp(min=0).long()
@@ -436,8 +435,7 @@ def _exact_select(s):
     bs, hkv, G, k = case["block"], case["kv_heads"], case["heads"] // case["kv_heads"], case["select"]
     lens, off = s["lens"].tolist(), s["offsets"].tolist()
     q = s["q"].float()
-    size = q.abs().amax(-1, keepdim=True)
-    size = size / torch.full_like(size, 127.0)
+    size = q.abs().amax(-1, keepdim=True) / 127
     c = (q * (1 / size)).round()
     out = torch.full((q.shape[0], hkv, k), -1, dtype=torch.int32, device="cuda")
     for b, n in enumerate(lens):
