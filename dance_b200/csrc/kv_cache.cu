@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(D / 8 * kTokenGroups, IT <= 2 ? 1536 / (D / 8 
                 }
             }
         }
-    float amax[2];
+    float largest[2];
     bool odd = false; // infinities or NaN among the thread's values
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind)
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(D / 8 * kTokenGroups, IT <= 2 ? 1536 / (D / 8 
             top = max_u16x2(top, max_u16x2(x[kind][i].z & 0x7FFF7FFFu, x[kind][i].w & 0x7FFF7FFFu));
         }
         const uint32_t most = max(top & 0xFFFFu, top >> 16);
-        amax[kind] = kv_float<BF16>((uint16_t)most);
+        largest[kind] = kv_float<BF16>((uint16_t)most);
         odd |= most >= (BF16 ? 0x7F80u : 0x7C00u);
     }
     if (odd)
@@ -185,13 +185,13 @@ __global__ void __launch_bounds__(D / 8 * kTokenGroups, IT <= 2 ? 1536 / (D / 8 
 #pragma unroll
         for (int kind = 0; kind < 2; ++kind)
         {
-            amax[kind] = 0.0f;
+            largest[kind] = 0.0f;
 #pragma unroll
             for (int i = 0; i < IT; ++i)
-                amax[kind] = fmaxf(amax[kind], finite_max<BF16>(x[kind][i]));
+                largest[kind] = fmaxf(largest[kind], finite_max<BF16>(x[kind][i]));
         }
     }
-    const float2 both = block_max(make_float2(amax[0], amax[1]), red);
+    const float2 both = block_max(make_float2(largest[0], largest[1]), red);
 
     uint32_t lo4[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, hi4[2] = {0u, 0u};
     float key_shrink = 1.0f;
@@ -199,11 +199,14 @@ __global__ void __launch_bounds__(D / 8 * kTokenGroups, IT <= 2 ? 1536 / (D / 8 
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind)
     {
-        const float scale = fmaxf(old[kind], kv_scale_of(kind ? both.y : both.x));
-        const float inv = kv_inverse(scale);
+        const float amax = kind ? both.y : both.x, quotient = kv_scale_of(amax);
+        const float scale = fmaxf(old[kind], quotient);
+        // written again (quotient == old), the same rows get the same codes
+        const float step = old[kind] > quotient ? old[kind] : kv_step_of(amax);
+        const float inv = kv_inverse(step);
         // a scale that was never written (NaN) cannot be told from a grown one: the comparison treats it as grown
         const bool grew = n_old > 0 && !(scale == old[kind]);
-        const float shrink = scale > 0.0f ? __fdiv_rn(old[kind], scale) : 0.0f;
+        const float shrink = step > 0.0f ? __fdiv_rn(old[kind], step) : 0.0f;
         uint8_t *codes = (kind ? p.c.v + (uint64_t)blk * p.c.vbs : p.c.k + (uint64_t)blk * p.c.kbs) +
                          (uint64_t)h * (kBs * D) + d8 * 8;
 #pragma unroll

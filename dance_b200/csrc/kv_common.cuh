@@ -108,10 +108,22 @@ __device__ __forceinline__ uint32_t kv_pack(float lo, float hi)
 }
 
 // Scale of a set of finite magnitudes, and the code - 128 of a value at a
-// scale: 1/scale is taken once per scale, so that a value costs one product.
+// step: 1/step is taken once, so that a value costs one product.
+//
+// The scale is the quotient amax / 127, the float nearest to it.  The step that
+// codes are taken at is amax times the float nearest 1/127: the scale, or, for
+// 4.6 % of all magnitudes, the float below it.  Where the two part, so do their
+// codes only at half the magnitude, whose exact code 63.5 is a tie: the step
+// gives the even 64, the scale for half of these magnitudes 63 (every pair of
+// float16 and of bfloat16 numbers was compared with the exact quotient).
 __device__ __forceinline__ float kv_scale_of(float amax)
 {
     const float s = __fdiv_rn(amax, 127.0f);
+    return s < kKvTiny ? 0.0f : s;
+}
+__device__ __forceinline__ float kv_step_of(float amax)
+{
+    const float s = __fmul_rn(amax, 1.0f / 127.0f);
     return s < kKvTiny ? 0.0f : s;
 }
 __device__ __forceinline__ float kv_inverse(float s) { return s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f; }

@@ -503,8 +503,12 @@ typedef struct DanceKvRows
  * block and head, with x the new rows that fall into it:
  *   scale' = max(scale if the block held tokens of the sequence before,
  *                max |x| over finite x / 127), below 2^-126: 0;
- *   codes held before: rint((c - 128) * (scale / scale')) + 128;
- *   new codes: clamp(rint(x * (1 / scale')), -127, 127) + 128, NaN -> 128;
+ *   step = scale where it is larger than that quotient, else max |x| times
+ *          the float nearest 1/127 (scale' or the float below it), below
+ *          2^-126: 0;
+ *   codes held before: rint((c - 128) * (scale / step)) + 128 where scale' is
+ *          larger than scale;
+ *   new codes: clamp(rint(x * (1 / step)), -127, 127) + 128, NaN -> 128;
  * in float, ties to even.  The bounds of a block that held tokens before are
  * rounded as its codes are, and widened by the new codes; a block's first
  * tokens set them.  (Rows may be written again at shorter lengths, as after a
