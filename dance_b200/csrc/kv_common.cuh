@@ -110,7 +110,7 @@ __device__ __forceinline__ uint32_t kv_pack(float lo, float hi)
 // Scale of a set of finite magnitudes, and the code - 128 of a value at a
 // step: 1/step is taken once, so that a value costs one product.
 //
-// The scale is the quotient amax / 127, the float nearest to it.  The step that
+// A block's scale is the quotient amax / 127, the float nearest to it.  The step that
 // codes are taken at is amax times the float nearest 1/127: the scale, or, for
 // 4.6 % of all magnitudes, the float below it.  Where the two part, so do their
 // codes only at half the magnitude, whose exact code 63.5 is a tie: the step

@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) scores_kernel(SelectParams p
                     const unsigned eight = 0xFFu << (threadIdx.x & 24);
                     for (int o = 4; o; o >>= 1)
                         amax = fmaxf(amax, __shfl_xor_sync(eight, amax, o));
-                    const float qs = kv_scale_of(amax), inv = kv_inverse(qs);
+                    const float qs = kv_step_of(amax), inv = kv_inverse(qs);
                     int sum = 0;
                     uint8_t *dst = smem + (hd * kRows + e % kRows) * kStride + l8 * (D / 8);
 #pragma unroll

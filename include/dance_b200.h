@@ -541,8 +541,8 @@ DANCE_API int dance_kv_attention(const DanceKvCache *cache, const DanceKvBatch *
  * rest up to select in all, by the score
  *   max over the head's query heads of  s_q * B  times the block's key scale,
  *   B = sum_d max(c_d * (low_d - 128), c_d * (high_d - 128)),
- * c = clamp(rint(q * (1 / s_q)), -127, 127), s_q = max |q| over finite q / 127
- * (below 2^-126: 0), low and high the block's bounds.  B is an integer; the
+ * c = clamp(rint(q * (1 / s_q)), -127, 127), s_q = max |q| over finite q times
+ * the float nearest 1/127 (below 2^-126: 0), low and high the block's bounds.  B is an integer; the
  * two products are float, in this order.  Ties go to the lower block.
  * select >= first_blocks + last_blocks, 1 <= select <= 4096. */
 DANCE_API int dance_kv_select_blocks(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *q,

@@ -101,3 +101,25 @@ def test_append_codes_are_those_of_the_step(dance_lib, dim, bs, dtype):
         assert np.array_equal(t.cpu().numpy().astype(int) - 128, want.astype(int))
     b = cache.bounds.cpu().numpy().astype(int) - 128
     assert np.array_equal(b[:, :, 0], want.min(2)) and np.array_equal(b[:, :, 1], want.max(2))
+
+
+# ------------------------------------------------------------------ selection
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_selection_rounds_ties_to_even(dance_lib, dtype):
+    """Two blocks whose bounds weigh a query's tied channel against its largest one: the code of the tie decides."""
+    import torch
+    from dance_b200 import kvcache
+    most = magnitudes(dtype)
+    T = len(most)
+    cache = kvcache.KVCache.create(4, 1, 64, 16)
+    # scores of blocks 1 and 2: 127 * 63 and 64 * 126 (+ 62 of a channel of code 1), so that code 63 would choose block 1
+    cache.bounds[1, 0, :, 0] = 128 + 63
+    cache.bounds[2, 0, :, 1] = 128 + 126
+    cache.k_scale.fill_(0.5)
+    q = np.zeros((T, 1, 64), np.float32)
+    q[:, 0, 0], q[:, 0, 1] = most, most / 2
+    assert 127 * 63 < 64 * 126 and 127 * 63 > 63 * 126
+    t = torch.tensor(q, device="cuda").to(getattr(torch, dtype))
+    got = kvcache.select_blocks(cache, batch_of([[0, 1, 2, 3]] * T, [64] * T, [1] * T), t, 3)
+    assert np.array_equal(got.cpu().numpy()[:, 0], np.tile([0, 2, 3], (T, 1)))
