@@ -136,29 +136,76 @@ class KVBatch:
 
 class KVWorkspace:
     """Device scratch of the attention and the selection, grown on demand; it
-    serves one call at a time (calls on one stream, say)."""
+    serves one call at a time (calls on one stream, or on streams that wait for
+    one another).
+
+    Buffers that it outgrew stay allocated as long as it lives: a CUDA graph
+    that was captured with one still writes to it, and so may a call in flight.
+    Each is at least twice as large as the one before, so that all of them
+    together take less than the last one again.
+    """
 
     def __init__(self):
-        self._t = None
+        self._held: dict = {}  # device -> its buffers, the last in use
+        self._index = None     # device of the buffer in use
         self._ptr = 0
         self._bytes = 0
         self._known = set()
+        self._stream = None    # the stream that last came behind the zeroing
+        self._zeroed = None
 
     def reserve(self, cache: KVCache, batch: KVBatch, rows: int, num_heads: int, select: int = 0) -> None:
-        """Room for such a call (before a stream capture, which must not allocate)."""
-        key = (cache._key, batch._key, rows, num_heads, select)
-        if key not in self._known:
-            need = load().dance_kv_workspace_bytes(cache._ptr, batch._ptr, rows, num_heads, select)
-            if need == 0:
-                check(-1, "dance_kv_workspace_bytes")
-            if need > self._bytes or self._t.device != cache.device:
-                import torch
-                self._t = torch.zeros(need, dtype=torch.uint8, device=cache.device)
-                self._ptr, self._bytes = self._t.data_ptr(), need
-                self._known.clear()  # what it held room for may have been on another device
-            if len(self._known) > 256:
-                self._known.clear()
-            self._known.add(key)
+        """Room for such a call.  A workspace does not grow in a stream capture, where its zeroing would wait for the
+        graph's replay: reserve before, and let that finish."""
+        if (cache._key, batch._key, rows, num_heads, select) not in self._known:
+            import torch
+            self._grow(cache, batch, rows, num_heads, select, not torch.cuda.is_current_stream_capturing())
+
+    def _grow(self, cache, batch, rows, num_heads, select, may_allocate):
+        need = load().dance_kv_workspace_bytes(cache._ptr, batch._ptr, rows, num_heads, select)
+        if need == 0:
+            check(-1, "dance_kv_workspace_bytes")
+        if self._index != cache._index:
+            self._index, self._bytes, self._stream = cache._index, 0, None
+            self._known.clear()
+            if self._index in self._held:
+                self._set(*self._held[self._index][-1])
+        if need > self._bytes:
+            import torch
+            _need(may_allocate, f"the workspace holds {self._bytes} bytes, {need} are needed: "
+                                "reserve them before the stream capture")
+            with torch.cuda.device(cache.device):
+                t = torch.zeros(max(need, 2 * self._bytes), dtype=torch.uint8, device=cache.device)
+                done = torch.cuda.Event()
+                done.record()
+                self._stream = torch.cuda.current_stream().cuda_stream
+            self._held.setdefault(self._index, []).append((t, done))
+            self._set(t, done)
+        if len(self._known) > 256:
+            self._known.clear()
+        self._known.add((cache._key, batch._key, rows, num_heads, select))
+
+    def _set(self, t, done):
+        self._ptr, self._bytes, self._zeroed = t.data_ptr(), t.numel(), done
+
+    def _follow(self, stream):
+        """Lets the current stream, of that handle, wait for the buffer's zeroing."""
+        import torch
+        if not torch.cuda.is_current_stream_capturing():  # before a capture the caller waits
+            torch.cuda.current_stream().wait_event(self._zeroed)
+            self._stream = stream
+
+
+def _scratch(workspace, cache, batch, rows, heads, select, stream):
+    """The workspace of a call on the current stream, with room for it; a new one where the caller has none."""
+    if workspace is None:
+        workspace = KVWorkspace()
+        workspace._grow(cache, batch, rows, heads, select, True)  # in a capture it is the graph's, zeroed by each replay
+    else:
+        workspace.reserve(cache, batch, rows, heads, select)
+        if workspace._stream != stream:
+            workspace._follow(stream)
+    return workspace
 
 
 # The calls below are short (a decode step calls them once per layer), so what
@@ -281,8 +328,7 @@ def _attend(cache, batch, q, blocks, scale, return_lse, out, workspace):
             raise ValueError("blocks must be contiguous, on the cache's device")
         if not 1 <= select <= 4096:
             raise ValueError(f"{select} blocks per row: 1 to 4096 are supported")
-    ws = workspace or KVWorkspace()
-    ws.reserve(cache, batch, rows, heads, select)
+    ws = _scratch(workspace, cache, batch, rows, heads, select, stream)
     if scale is None:
         scale = dim ** -0.5
     if blocks is None:
@@ -335,8 +381,7 @@ def select_blocks(cache: KVCache, batch: KVBatch, q, select: int, *, first_block
     else:
         _cuda("out", out, _torch.int32, (rows, cache.kv_heads, select))
         _need(out.is_contiguous() and out.device == cache.device, "out must be contiguous, on the cache's device")
-    ws = workspace or KVWorkspace()
-    ws.reserve(cache, batch, rows, heads, select)
+    ws = _scratch(workspace, cache, batch, rows, heads, select, stream)
     rc = _lib.dance_kv_select_blocks(cache._ptr, batch._ptr, _address(qr), heads, select, first_blocks, last_blocks,
                                      out.data_ptr(), ws._ptr, ws._bytes, stream)
     if rc:

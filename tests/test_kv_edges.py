@@ -123,3 +123,88 @@ def test_selection_rounds_ties_to_even(dance_lib, dtype):
     t = torch.tensor(q, device="cuda").to(getattr(torch, dtype))
     got = kvcache.select_blocks(cache, batch_of([[0, 1, 2, 3]] * T, [64] * T, [1] * T), t, 3)
     assert np.array_equal(got.cpu().numpy()[:, 0], np.tile([0, 2, 3], (T, 1)))
+
+
+# ------------------------------------------------------------------ workspaces
+def decode_step(tokens, seed=0, heads=8):
+    """A call whose splits are joined through the workspace's counters."""
+    import torch
+    from dance_b200 import kvcache
+    n = -(-tokens // 64)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(1, 256, (2, n, 2, 64, 64), generator=g, device="cuda").to(torch.uint8)
+    scale = torch.full((2, n, 2), 0.01, device="cuda")
+    cache = kvcache.KVCache(codes[0], codes[1], scale[0], scale[1], codes[0, :, :, :2].contiguous())
+    q = torch.randn((1, heads, 64), generator=g, device="cuda").half()
+    return cache, batch_of([list(range(n))], [tokens], [1]), q
+
+
+@pytest.mark.gpu
+def test_captured_graph_survives_a_workspace_that_grows(dance_lib):
+    import torch
+    from dance_b200 import kvcache
+    cache, batch, q = decode_step(4000)
+    want = kvcache.attention(cache, batch, q)
+    ws = kvcache.KVWorkspace()
+    ws.reserve(cache, batch, 1, 8)
+    kvcache.attention(cache, batch, q, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kvcache.attention(cache, batch, q, workspace=ws)
+    small, address = ws._bytes, ws._ptr
+    big = decode_step(100000, heads=64)
+    large = kvcache.attention(*big, workspace=ws)
+    assert ws._bytes > small and ws._ptr != address
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    # what the allocator would hand out of a freed buffer
+    other = [torch.full((max(small // 2 ** i, 512),), 255, dtype=torch.uint8, device="cuda") for i in range(8) for _ in range(4)]
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(kvcache.attention(*big, workspace=ws), large)
+    assert all((t == 255).all() for t in other)
+
+
+@pytest.mark.gpu
+def test_workspace_does_not_grow_in_a_capture(dance_lib):
+    """Its zeroing would be the graph's: the call refuses.  A call without a workspace has one of the graph's own."""
+    import torch
+    from dance_b200 import kvcache
+    cache, batch, q = decode_step(4000)
+    want = kvcache.attention(cache, batch, q)
+    ws, graph = kvcache.KVWorkspace(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = kvcache.attention(cache, batch, q)
+        with pytest.raises(ValueError, match="before the stream capture"):
+            kvcache.attention(cache, batch, q, workspace=ws)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert torch.equal(kvcache.attention(cache, batch, q, workspace=ws), want)
+
+
+@pytest.mark.gpu
+def test_workspace_zeroed_on_another_stream(dance_lib):
+    """A workspace reserved on a busy stream is used on another one at once."""
+    import torch
+    from dance_b200 import kvcache
+    cache, batch, q = decode_step(4000)
+    want = kvcache.attention(cache, batch, q)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        ws = kvcache.KVWorkspace()
+        with torch.cuda.stream(a):
+            torch.full((64 << 20,), 255, dtype=torch.uint8, device="cuda")  # what the buffer may come out of
+            torch.cuda._sleep(20_000_000)
+            ws.reserve(cache, batch, 1, 8)
+        out = kvcache.attention(cache, batch, q, workspace=ws, stream=b)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
