@@ -25,7 +25,7 @@ SOURCES = ["vamana_build.cu", "vamana_sharded.cu", "gpu_merge.cu", "stitched.cu"
            "partition.cu", "kv_cache.cu", "kv_attention.cu", "kv_prompt.cu", "kv_select.cu"]
 HEADERS = ["dance_common.cuh", "vamana_kernels.cuh", "host_common.cuh", "filtered_kernels.cuh",
            "gram_u8.cuh", "prune_quad.cuh", "stitched_prune.cuh", "replay_umma.cuh", "comm.cuh",
-           "host_errors.cuh", "kv_common.cuh", "kv_attention.cuh"]
+           "host_errors.cuh", "func_attr.cuh", "kv_common.cuh", "kv_attention.cuh"]
 PUBLIC_HEADERS = ["dance_b200.h", "gpu_vamana_builder.h", "gpu_vamana_config.h", "gpu_merge.h",
                   "gpu_vamana_filtered.h"]
 

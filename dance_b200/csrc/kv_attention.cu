@@ -827,9 +827,8 @@ AttnPlan plan_attention(const DanceKvCache &c, const DanceKvBatch &b, uint32_t h
 template <int D, int NT, bool SPARSE, bool BF16>
 int launch_rows(const AttnParams &p, dim3 grid, cudaStream_t st)
 {
-    static const cudaError_t attr = cudaFuncSetAttribute(rows_kernel<D, NT, SPARSE, BF16>,
-                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem<D>());
-    DANCE_CUDA(attr);
+    static SmemAllowed allowed;
+    DANCE_CUDA(allowed.on_current(reinterpret_cast<const void *>(rows_kernel<D, NT, SPARSE, BF16>), rows_smem<D>()));
     rows_kernel<D, NT, SPARSE, BF16><<<grid, kWarps * 32, rows_smem<D>(), st>>>(p);
     DANCE_LAUNCHED();
     return 0;

@@ -15,6 +15,7 @@
 #include <cstdint>
 
 #include "../../include/dance_b200.h"
+#include "func_attr.cuh"
 #include "host_errors.cuh"
 
 namespace dance

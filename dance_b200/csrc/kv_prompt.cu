@@ -885,9 +885,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
 template <int D, bool BF16>
 int launch(const AttnParams &p, uint32_t blocks_x, cudaStream_t st)
 {
-    static const cudaError_t attr = cudaFuncSetAttribute(prompt_kernel<D, BF16>,
-                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::bytes);
-    DANCE_CUDA(attr);
+    static SmemAllowed allowed;
+    DANCE_CUDA(allowed.on_current(reinterpret_cast<const void *>(prompt_kernel<D, BF16>), Layout<D>::bytes));
     prompt_kernel<D, BF16><<<dim3(blocks_x, p.c.batch), kThreads, Layout<D>::bytes, st>>>(p);
     DANCE_LAUNCHED();
     return 0;

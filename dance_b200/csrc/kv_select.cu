@@ -628,14 +628,10 @@ int launch_scores(SelectParams &p, bool bf16, cudaStream_t st)
     // runs of one thread block: one, unless there is work for several waves without
     p.passes = (uint32_t)(tiles * runs >= 4 * 4 * 148 ? min(4u, runs) : 1u);
     const dim3 grid(p.row_tiles * ((runs + p.passes - 1) / p.passes), p.c.hkv, p.c.batch);
-    constexpr int per_head = 8 * NT * (code_stride<D>() + 8), most = kScoreHeads * per_head;
+    constexpr int per_head = 8 * NT * (code_stride<D>() + 8);
+    static_assert(kScoreHeads * per_head <= 48 * 1024, "more shared memory would have to be asked for");
     p.slots = min(p.G, (uint32_t)kScoreHeads);
     const int smem = (int)p.slots * per_head;
-    static const cudaError_t attr[2] = {
-        cudaFuncSetAttribute(scores_kernel<D, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most),
-        cudaFuncSetAttribute(scores_kernel<D, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)};
-    DANCE_CUDA(attr[0]);
-    DANCE_CUDA(attr[1]);
     if (bf16)
         scores_kernel<D, NT, true><<<grid, kScoreThreads, smem, st>>>(p);
     else

@@ -4,9 +4,8 @@ value, workspaces that grow, lists that share blocks.
 
 Expected values come from the formulas in 64 bits (or exact fractions), of the
 codes and scales that the cache holds, written apart from the kernels."""
-import ctypes
-import math
 from fractions import Fraction
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -125,6 +124,93 @@ def test_selection_rounds_ties_to_even(dance_lib, dtype):
     assert np.array_equal(got.cpu().numpy()[:, 0], np.tile([0, 2, 3], (T, 1)))
 
 
+# ------------------------------------------------------------------ attention
+class Held:
+    """A cache of given codes and scales, with the attention over it in 64 bits."""
+
+    def __init__(self, lens, rows, hkv, dim, bs, dtype, seed, k_scale=None, v_scale=None, table=None):
+        import torch
+        from dance_b200 import kvcache
+        rng = self.rng = np.random.default_rng(seed)
+        self.lens, self.rows, self.hkv, self.dim, self.bs, self.dtype = lens, rows, hkv, dim, bs, dtype
+        need = [-(-n // bs) for n in lens]
+        pool, width = sum(need) + 2, max(need)
+        ids = rng.permutation(pool)
+        self.table = np.full((len(lens), width), -1)
+        for b, n in enumerate(need):
+            self.table[b, :n] = ids[sum(need[:b]):sum(need[:b + 1])]
+        self.k = rng.integers(-127, 128, (pool, hkv, bs, dim))
+        self.v = rng.integers(-127, 128, (pool, hkv, bs, dim))
+        self.ks = np.full((pool, hkv), 0.02, np.float32) if k_scale is None else k_scale(self, pool)
+        self.vs = np.full((pool, hkv), 0.01, np.float32) if v_scale is None else v_scale(self, pool)
+        dev = [torch.tensor(x + 128, dtype=torch.uint8, device="cuda") for x in (self.k, self.v)]
+        bounds = torch.stack((dev[0].amin(2), dev[0].amax(2)), 2).contiguous()
+        self.cache = kvcache.KVCache(dev[0], dev[1], torch.tensor(self.ks, device="cuda"),
+                                     torch.tensor(self.vs, device="cuda"), bounds)
+        self.batch = batch_of(self.table, lens, rows)
+
+    def q(self, heads, size=1.0):
+        import torch
+        t = torch.tensor(self.rng.normal(size=(sum(self.rows), heads, self.dim)) * size, device="cuda")
+        t = t.to(getattr(torch, self.dtype))
+        return t, t.double().cpu().numpy()
+
+    def attention(self, q, scale, blocks=None):
+        """(out, lse, allowed error without the output's rounding, the lse's) in 64 bits.
+
+        Allowed: the weights' rounding to halves (2^-11), the logits' (products of D terms in float, S the largest sum
+        of magnitudes), 2^x and the sums in float (2^-19), each of sum_j p_j |v_j|; and what weights below a half's
+        range lose, 2^-30 of the row's largest p_j times its block's largest value, for each token."""
+        T, H, D = q.shape
+        G, bs = H // self.hkv, self.bs
+        out, lse, err = np.zeros((T, H, D)), np.full((T, H), -np.inf), np.zeros((T, H, D))
+        lse_err, r0 = np.zeros((T, H)), 0
+        for b, n in enumerate(self.lens):
+            rows, pages = self.rows[b], -(-n // bs)
+            at, place = self.table[b, :pages], np.arange(pages * bs)
+            for h in range(self.hkv):
+                times = np.ones((rows, pages)) if blocks is None else np.array(
+                    [[np.sum(blocks[r, h] == j) for j in range(pages)] for r in range(r0, r0 + rows)])
+                times = times.repeat(bs, 1) * (place <= n - rows + np.arange(rows)[:, None])  # how often a row sees a token
+                k = (self.k[at, h] * self.ks[at, h].astype(np.float64)[:, None, None]).reshape(-1, D)
+                v = (self.v[at, h] * self.vs[at, h].astype(np.float64)[:, None, None]).reshape(-1, D)
+                top = np.repeat(127 * self.vs[at, h].astype(np.float64), bs)
+                for g in range(h * G, (h + 1) * G):
+                    mine = slice(r0, r0 + rows)
+                    x = np.where(times > 0, scale * (q[mine, g] @ k.T), -np.inf)
+                    S = abs(scale) * np.where(times > 0, np.abs(q[mine, g]) @ np.abs(k).T, 0).max(1)
+                    most = x.max(1)
+                    p = times * np.exp(x - np.where(np.isinf(most), 0, most)[:, None])
+                    total = p.sum(1)
+                    some = total > 0
+                    lse[mine, g][some] = (most + np.log(np.where(some, total, 1)))[some]
+                    p /= np.where(some, total, 1)[:, None]
+                    out[mine, g] = p @ v
+                    lse_err[mine, g] = 2.0 ** -11 + 2 * (D + 8) * 2.0 ** -23 * S
+                    err[mine, g] = ((2.0 ** -11 + 2 * (D + 8) * 2.0 ** -23 * S + 2.0 ** -19)[:, None] * (p @ np.abs(v))
+                                    + (times.sum(1) * 2.0 ** -30 * (p * top).max(1))[:, None])
+            r0 += rows
+        return out, lse, err, lse_err
+
+
+def check_out(got, want, err, dtype):
+    u = 2.0 ** -11 if dtype == "float16" else 2.0 ** -8
+    # float16 has no numbers below 2^-24
+    err = err + (2.0 ** -25 if dtype == "float16" else 0.0)
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    excess = np.abs(got - want) - (u * np.abs(want) + err)
+    at = np.unravel_index(excess.argmax(), excess.shape)
+    assert excess.max() <= 0, f"{at}: {got[at]} where {want[at]} +- {err[at]} is right"
+
+
+def check_lse(got, want, err):
+    got = got.double().cpu().numpy()
+    none = np.isinf(want)
+    assert np.array_equal(np.isneginf(got), none)
+    assert (np.abs(got[~none] - want[~none]) <= err[~none]).all()
+
+
 # ------------------------------------------------------------------ workspaces
 def decode_step(tokens, seed=0, heads=8):
     """A call whose splits are joined through the workspace's counters."""
@@ -208,3 +294,66 @@ def test_workspace_zeroed_on_another_stream(dance_lib):
         out = kvcache.attention(cache, batch, q, workspace=ws, stream=b)
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------ several devices
+FAKE_RUNTIME = r'''
+#include "func_attr.cuh"
+#include <cstdio>
+static int device, fails, asked[2];
+extern "C" cudaError_t cudaGetDevice(int *d) { *d = device; return cudaSuccess; }
+extern "C" cudaError_t cudaFuncSetAttribute(const void *, cudaFuncAttribute, int bytes)
+{
+    ++asked[device];
+    return fails && fails-- ? cudaErrorInvalidValue : bytes == 70000 ? cudaSuccess : cudaErrorUnknown;
+}
+int main()
+{
+    static dance::SmemAllowed a;
+    fails = 1;
+    const cudaError_t first = a.on_current(nullptr, 70000), second = a.on_current(nullptr, 70000);
+    cudaError_t later = a.on_current(nullptr, 70000);
+    device = 1;
+    const cudaError_t other = a.on_current(nullptr, 70000);
+    for (device = 0; device < 2; ++device)
+        later = a.on_current(nullptr, 70000);
+    printf("%d %d %d %d %d %d\n", first != cudaSuccess, second, other, later, asked[0], asked[1]);
+}
+'''
+
+
+def test_shared_memory_is_asked_for_on_every_device(tmp_path):
+    """Against a fake of the runtime with two devices: once on each, again after a failure."""
+    import shutil
+    import subprocess
+    from dance_b200 import build
+    nvcc = build.nvcc()
+    root = Path(shutil.which(nvcc) or nvcc).resolve().parent.parent
+    (tmp_path / "t.cpp").write_text("#include <cuda_runtime_api.h>\n" + FAKE_RUNTIME)
+    exe = tmp_path / "t"
+    subprocess.run(["g++", "-std=c++17", "-I", str(root / "include"), "-I", str(build.CSRC), str(tmp_path / "t.cpp"),
+                    "-o", str(exe)], check=True)
+    assert subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split() == list("100021")
+
+
+def test_no_attribute_is_remembered_for_the_process():
+    from dance_b200 import build
+    for src in build.SOURCES:
+        text = (build.CSRC / src).read_text()
+        assert "static const cudaError_t" not in text, src
+
+
+@pytest.mark.gpu
+def test_attention_on_a_second_device(dance_lib):
+    import torch
+    from dance_b200 import kvcache
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    for rows in (1, 40):
+        outs = []
+        for dev in (0, 1):
+            with torch.cuda.device(dev):
+                w = Held([300], [rows], 1, 128, 64, "float16", seed=rows)
+                q, _ = w.q(2)
+                outs.append(kvcache.attention(w.cache, w.batch, q).cpu())
+        assert torch.equal(*outs)
