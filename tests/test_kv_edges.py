@@ -10,6 +10,8 @@ from pathlib import Path
 import numpy as np
 import pytest
 
+import test_kvcache
+
 DTYPES = ("float16", "bfloat16")
 STEP = np.float32(1) / np.float32(127)
 
@@ -122,6 +124,115 @@ def test_selection_rounds_ties_to_even(dance_lib, dtype):
     t = torch.tensor(q, device="cuda").to(getattr(torch, dtype))
     got = kvcache.select_blocks(cache, batch_of([[0, 1, 2, 3]] * T, [64] * T, [1] * T), t, 3)
     assert np.array_equal(got.cpu().numpy()[:, 0], np.tile([0, 2, 3], (T, 1)))
+
+
+# ------------------------------------------------------------------ the twin on the host, by the step
+class StepCache(test_kvcache.PlainCache):
+    """The cache on the host with codes at the step: half of a block's largest magnitude, an exact 63.5, is 64."""
+
+    def append(self, table, lens, offsets, k, v):
+        quotient, codes = test_kvcache.plain_scale, test_kvcache.plain_codes
+        for b, n in enumerate(lens):
+            first = n - (offsets[b + 1] - offsets[b])
+            for page in range(max(first, 0) // self.bs, -(-n // self.bs) if n > 0 else 0):
+                lo, hi = max(first, 0, page * self.bs), min(n, (page + 1) * self.bs)
+                at = table[b][page] if page < len(table[b]) else -1
+                if hi <= lo or not 0 <= at < self.n:
+                    continue
+                begun, end = lo - page * self.bs, hi - page * self.bs
+                for h in range(self.hkv):
+                    for name, x in (("k", k), ("v", v)):
+                        new = x[offsets[b] + lo - first:offsets[b] + hi - first, h]
+                        old = self.scale[name][at, h] if begun else np.float32(0)
+                        largest = quotient(new)
+                        step = old if old > largest else step_of(new)
+                        c, ends = self.code[name][at, h], np.stack((self.low[at, h], self.high[at, h]))
+                        if begun and largest > old:
+                            c[:begun] = np.rint(c[:begun].astype(np.float32) * (old / step))
+                            ends = np.rint(ends.astype(np.float32) * (old / step)).astype(np.int64)
+                        c[begun:end] = codes(new, step)
+                        self.scale[name][at, h] = max(old, largest)
+                        if name == "k":
+                            low, high = c[begun:end].min(0), c[begun:end].max(0)
+                            self.low[at, h] = np.minimum(ends[0], low) if begun else low
+                            self.high[at, h] = np.maximum(ends[1], high) if begun else high
+
+
+def step_of(x):
+    """The step of a set of values: the largest finite |x| times the float nearest 1/127."""
+    a = np.abs(x[np.isfinite(x)])
+    s = np.float32(a.max() if a.size else 0.0) * STEP
+    return np.float32(0.0) if s < np.float32(2.0 ** -126) else s
+
+
+@pytest.fixture
+def twin(monkeypatch):
+    monkeypatch.setattr(test_kvcache, "PlainCache", StepCache)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,bs", [(64, 16), (96, 32), (128, 64), (64, 128), (128, 16), (96, 128)])
+def test_append_equals_the_twin(dance_lib, twin, dim, bs, dtype):
+    test_kvcache.test_append_equals_the_definition(dance_lib, dim, bs, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_of_odd_values_equals_the_twin(dance_lib, twin, dtype):
+    test_kvcache.test_append_odd_values(dance_lib, dtype)
+
+
+@pytest.mark.gpu
+def test_append_token_by_token_equals_the_twin(dance_lib, twin):
+    test_kvcache.test_append_token_by_token(dance_lib)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", test_kvcache.SHAPES)
+def test_attention_over_the_twin(dance_lib, twin, shape, dtype):
+    test_kvcache.test_attention_against_64_bits(dance_lib, shape, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", test_kvcache.SHAPES)
+@pytest.mark.parametrize("select", (4, 11))
+def test_sparse_attention_over_the_twin(dance_lib, twin, shape, dtype, select):
+    test_kvcache.test_sparse_attention_against_64_bits(dance_lib, shape, dtype, select)
+
+
+class QuotientFirst(StepCache):
+    """StepCache where the module's scale of a set of values is the step, as a query's is."""
+
+    def append(self, *args):
+        with pytest.MonkeyPatch.context() as m:
+            m.setattr(test_kvcache, "plain_scale", PLAIN_SCALE)
+            super().append(*args)
+
+
+PLAIN_SCALE = test_kvcache.plain_scale
+
+
+@pytest.fixture
+def select_twin(monkeypatch):
+    monkeypatch.setattr(test_kvcache, "PlainCache", QuotientFirst)
+    monkeypatch.setattr(test_kvcache, "plain_scale", step_of)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", test_kvcache.SELECTS)
+def test_selection_equals_the_twin(dance_lib, select_twin, case, dtype):
+    test_kvcache.test_selection_equals_the_definition(dance_lib, case, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,G", [(1, 4), (12, 3)])
+def test_selection_of_a_long_sequence_equals_the_twin(dance_lib, select_twin, rows, G):
+    for _ in range(4):
+        test_kvcache.test_selection_of_a_long_sequence(dance_lib, rows, G)
 
 
 # ------------------------------------------------------------------ attention
