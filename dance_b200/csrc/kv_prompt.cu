@@ -403,7 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         for (int e = 0; e < D / 2; ++e)
             amax = fmaxf(amax, fmaxf(fabsf(kv_float<BF16>((uint16_t)x[e])), fabsf(kv_float<BF16>((uint16_t)(x[e] >> 16)))));
         const int up = row_shift(amax);
-        const float mul = power_of_two(up);
+        // the sign of the logits' factor goes into q: a group's largest logit has to be that of its largest product
+        const float mul = p.scale_log2 < 0.0f ? -power_of_two(up) : power_of_two(up);
 #pragma unroll
         for (int c = 0; c < D / 8; ++c)
         {
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             *reinterpret_cast<uint4 *>(smem + L::q + (tid >> 7) * L::kTileBytes + tile_off(tid & 127, c)) =
                 make_uint4(y[0], y[1], y[2], y[3]);
         }
-        rf = live ? power_of_two(-up) * p.scale_log2 : 0.0f;
+        rf = live ? power_of_two(-up) * fabsf(p.scale_log2) : 0.0f;
         limit = live ? min(w.s.first + i + 1, w.s.len) : 0;
         fence_smem();
     }

@@ -525,7 +525,8 @@ DANCE_API int dance_kv_read(const DanceKvCache *cache, const DanceKvBatch *batch
 /* Attention of the rows q (rows x num_heads; num_heads a multiple of
  * kv_heads, query head h reading key/value head h / (num_heads / kv_heads))
  * over their sequences' tokens up to their own position:
- *   out = sum_j softmax_j(scale * q.k_j) v_j.
+ *   out = sum_j softmax_j(scale * q.k_j) v_j,
+ * scale any finite number.
  * d_out: rows x num_heads x head_dim of q's type, contiguous, 16-byte
  * aligned; d_lse (optional): log sum_j exp(scale * q.k_j), rows x num_heads.
  * A row that sees no token gets 0 and -inf.  d_workspace holds at least

@@ -322,6 +322,23 @@ def check_lse(got, want, err):
     assert (np.abs(got[~none] - want[~none]) <= err[~none]).all()
 
 
+ROWS = (1, 5, 40, 300)  # of a sequence: few rows, drafts, one row tile, two
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("scale", (-0.1, 0.0, 0.1, -3.0))
+def test_attention_factor_of_any_sign(dance_lib, rows, scale, dtype):
+    from dance_b200 import kvcache
+    w = Held([700, 333], [rows, 1], 1, 128, 64, dtype, seed=rows)
+    q, qn = w.q(2)
+    out, lse = kvcache.attention(w.cache, w.batch, q, scale, return_lse=True)
+    want, want_lse, err, lse_err = w.attention(qn, scale)
+    check_out(out, want, err, dtype)
+    check_lse(lse, want_lse, lse_err)
+
+
 # ------------------------------------------------------------------ workspaces
 def decode_step(tokens, seed=0, heads=8):
     """A call whose splits are joined through the workspace's counters."""
