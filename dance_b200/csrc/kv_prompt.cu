@@ -13,7 +13,7 @@
 // columns of S, 2 x 64 of P, 2 x head_dim of O, full at 128 channels.
 //
 // Measured on 2594 rows x 32 heads over 16000 and 7100 tokens of 128 channels:
-// 0.78 ms, 0.72 PFLOP/s (0.43 of the measured matrix rate).  A token tile takes
+// 0.77 ms, 0.73 PFLOP/s (0.44 of the measured matrix rate).  A token tile takes
 // about 4900 clocks where the tensor core works 2100: what bounds it are the
 // softmax threads' 3200 clocks for a tile (two warps a scheduler, the
 // exponentials half of it) and the turning of codes into halves; tensor core,
@@ -35,9 +35,15 @@
 // row, with a 128-byte swizzle; K is read as K-major, V, whose rows are the
 // summed dimension, as MN-major.  Warp 12 issues the matrix instructions.
 //
-// Rescaling O in tensor memory is a round trip, so a row keeps its reference
-// maximum until the true one exceeds it by 2^8: weights are 2^(s - ref + 7) <=
-// 2^15, inside a half.  The reference only shifts weights and their sum alike.
+// Weights.  A row sums p = 2^(s - m) in float; the product's operand is the half
+// of p sv 2^base.  Rescaling O in tensor memory is a round trip, so m and base
+// stay until a logit exceeds m by 8 or a weight would pass 2^15.  base is then set so
+// that the row's largest p sv becomes 2^6 to 2^7: a weight has its 11 bits down to
+// 2^-20 of the row's largest p sv and is lost below 2^-31.  Both come from the
+// tokens that the row sees alone, however far apart the blocks' value scales lie;
+// m and base are whole numbers, which sums and outputs are scaled by exactly.
+// (Weights taken relative to the split's largest value scale, with no base to
+// keep, were no faster: 783 us for the call above, against 774.)
 //
 // Every wait on a barrier is bounded.  A block that gives up counts itself in
 // g_kv_prompt_timeouts, and its rows read as not-a-number.
@@ -65,8 +71,11 @@ constexpr int kSoftRegs = 184, kConvRegs = 96, kMmaRegs = 48;
 constexpr int kTok = (int)kPromptTokens;
 constexpr int kGroups = kTok / 16;    // 16 tokens share a cache block
 constexpr int kFactorStages = 4;      // factors are read up to two tiles after the codes are free
-constexpr float kLift = 7.0f;         // log2 of the weight of a row's reference maximum
-constexpr float kSlack = 8.0f;        // how far the maximum may rise above the reference
+constexpr float kLift = 7.0f;         // log2 of a row's largest weight when its base is set
+constexpr float kSlack = 8.0f;        // how far maximum and weights may rise before they are set anew
+constexpr float kMostBase = 126.0f;   // bases whose power of two, and its inverse, are normal numbers
+constexpr float kTame = 24.0f, kTameBase = 48.0f; // log2 of value scales, and bases, of a plain tile, up and down
+constexpr float kFar = 1048576.0f;    // logits beyond it: their unrounded products part from the rounded ones
 constexpr uint32_t kWaitNs = 20000;           // how long one try may sleep
 constexpr long long kWaitClocks = 2000000000; // about a second: a wait in earnest is over in microseconds
 
@@ -78,7 +87,8 @@ struct Layout
     static constexpr int k = 2 * kTileBytes;        // two stages
     static constexpr int v = 4 * kTileBytes;        // two stages
     static constexpr int factors = 6 * kTileBytes;  // kFactorStages x kGroups x (logit factor, log2 of the
-                                                    // weight's factor, position, its inverse)
+                                                    // value scale, position (with the sign where the scale is far from
+                                                    // 1), inverse of the value scale)
     static constexpr int bars = factors + kFactorStages * kGroups * 16;
     static constexpr int misc = bars + 24 * 8;
     static constexpr int used = misc + 64 + 1024;
@@ -328,7 +338,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
     volatile int *gave_up = reinterpret_cast<volatile int *>(smem + L::misc);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::misc + 4);
     int *s_last = reinterpret_cast<int *>(smem + L::misc + 8);
-    uint32_t *s_vmax = reinterpret_cast<uint32_t *>(smem + L::misc + 12);
     float4 *s_f = reinterpret_cast<float4 *>(smem + L::factors);
 
     if (warp == kMmaWarp)
@@ -354,27 +363,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         bar_init(bar(kDrain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         *gave_up = 0;
-        *s_vmax = 0u;
     }
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_slot;
-
-    // ---- the largest value scale of the split: weights are taken relative to it
-    {
-        float vm = 0.0f;
-        for (int e = w.e0 + tid; e < w.e1; e += kThreads)
-        {
-            const int blk = kv_block(p.c, w.b, e);
-            if (blk >= 0)
-                vm = fmaxf(vm, __ldg(p.c.vs + (uint64_t)blk * p.c.hkv + w.h));
-        }
-        for (int o = 16; o; o >>= 1)
-            vm = fmaxf(vm, __shfl_xor_sync(kKvFull, vm, o));
-        if (lane == 0 && vm > 0.0f)
-            atomicMax(s_vmax, __float_as_uint(vm));
-    }
 
     // ---- q: one thread per row, as halves
     float rf = 0.0f; // logit factor of the thread's row
@@ -421,8 +414,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         fence_smem();
     }
     __syncthreads();
-    const float vref = __uint_as_float(*s_vmax);
-    float m = kKvNegInf, l = 0.0f;
+    float m = kKvNegInf, l = 0.0f, base = kMostBase, unbase = 0.0f;
+    float limit_w = kKvNegInf; // of a logit plus log2 of its value scale, until base is set anew
     bool ok = true;
 
     if (warp < kSoftWarps)
@@ -452,12 +445,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             bool whole = w.base + (i + 1) * kTok <= tile_lo;
 #pragma unroll
             for (int g = 0; g < kGroups; ++g)
-                whole &= __float_as_int(f[g].z) != kMaxPos;
+                whole &= __float_as_uint(f[g].z) < (uint32_t)kMaxPos;
             tmem_ld_wait(x[0]);
             loaded(x[1]);
             tmem_ld32(s_addr + 64u, x[2]);
             tmem_ld32(s_addr + 96u, x[3]);
-            float top = kKvNegInf;
+            float top = kKvNegInf, heavy = kKvNegInf; // largest logit; largest logit plus log2 of its value scale
             // the logits' factor is not negative and constant over 16 tokens
             auto maximum = [&](auto masked, int g0) {
 #pragma unroll
@@ -465,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 {
                     const float4 fg = f[g];
                     float m0 = kKvNegInf, m1 = kKvNegInf;
-                    const int left = limit - __float_as_int(fg.z); // columns of the group that the row sees
+                    const int left = limit - (__float_as_int(fg.z) & kMaxPos); // columns of the group that the row sees
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                     {
@@ -475,13 +468,18 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                         m1 = fmaxf(m1, !masked || e + 8 < left ? y1 : kKvNegInf);
                     }
                     m0 = fmaxf(m0, m1);
+                    float y = m0 * (fg.x * rf);
                     if constexpr (masked)
-                        top = fmaxf(top, m0 == kKvNegInf ? kKvNegInf : m0 * (fg.x * rf));
-                    else
-                        top = fmaxf(top, m0 * (fg.x * rf));
+                        y = m0 == kKvNegInf ? kKvNegInf : y;
+                    top = fmaxf(top, y);
+                    heavy = fmaxf(heavy, y + fg.y);
                 }
             };
-            auto weights = [&](auto masked, float shift_m) {
+            // Weights p = 2^(s - m), summed, and p times value scale times 2^base, the product's operand.  Plain tiles
+            // take the latter's exponent at once and the sum's terms from it; where a mask, far logits or a scale
+            // that would leave the range of floats there are met, each is computed by itself.
+            auto weights = [&](auto masked) {
+                const float shift_m = masked && m == kKvNegInf ? 0.0f : -m;
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                 {
@@ -490,8 +488,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                     for (int u = 0; u < 2; ++u)
                     {
                         const float4 fg = f[2 * c + u];
-                        const float kf = fg.x * rf, sm = shift_m + fg.y;
-                        const int left = limit - __float_as_int(fg.z);
+                        const float kf = fg.x * rf, sm = masked ? shift_m : shift_m + (base + fg.y);
+                        const float vf = masked ? exp2_fast(fminf(base + fg.y, kMostBase)) : 1.0f;
+                        const int left = limit - (__float_as_int(fg.z) & kMaxPos);
                         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
@@ -503,8 +502,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                             {
                                 // cut off what the exponent's unrounded product exceeds the maximum by; a logit
                                 // that is not a number stays one
-                                z.x = z.x > kLift + kSlack ? kLift + kSlack : z.x;
-                                z.y = z.y > kLift + kSlack ? kLift + kSlack : z.y;
+                                z.x = z.x > kSlack ? kSlack : z.x;
+                                z.y = z.y > kSlack ? kSlack : z.y;
                                 z.x = 2 * e < left ? z.x : kKvNegInf;
                                 z.y = 2 * e + 1 < left ? z.y : kKvNegInf;
                             }
@@ -512,9 +511,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                             z.y = exp2_fast(z.y);
                             sum.x += z.x;
                             sum.y += z.y;
+                            if constexpr (masked)
+                                z.x *= vf, z.y *= vf;
                             y[8 * u + e] = kv_pack<false>(z.x, z.y);
                         }
-                        l = fmaf(sum.x + sum.y, fg.w, l);
+                        l = masked ? l + (sum.x + sum.y) : fmaf(sum.x + sum.y, fg.w * unbase, l);
                     }
                     tmem_st16(p_addr + 16u * c, y);
                 }
@@ -542,13 +543,30 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 }
                 fence_after();
             }
-            const bool rise = top > m + kSlack; // from -inf: any maximum
-            if (__any_sync(kKvFull, rise))
+            if (__any_sync(kKvFull, top > m + kSlack || heavy > limit_w))
             {
-                const float down = !rise ? 1.0f : exp2_fast(m - top); // from -inf: 0
-                m = rise ? top : m;
-                l *= down;
-                if (i > 0)
+                // m: an integer, so that powers of two are all that sums and outputs are scaled by
+                const float mn = top > m + kSlack ? ceilf(top) : m; // from -inf: any maximum
+                const bool far = fabsf(mn) >= kFar && mn != kKvNegInf;
+                float need = heavy - mn; // log2 of the largest p times value scale
+                if (__any_sync(kKvFull, far))
+                {
+                    // where the sum's rounding hides the scale: the tile's largest, with the most that p can be
+                    float most = kKvNegInf;
+#pragma unroll 1
+                    for (int g = 0; g < kGroups; ++g)
+                        most = fmaxf(most, f[g].y);
+                    need = far ? kSlack + most : need;
+                }
+                const float keep = fminf(base + (mn - m), kMostBase); // leaves O as it is; from -inf: kMostBase
+                const float bn = need + keep > kLift + kSlack ? fmaxf(floorf(kLift - need), -kMostBase) : keep;
+                const float out_down = mn != m || bn != base ? exp2_fast((m - mn) + (bn - base)) : 1.0f;
+                l *= mn != m ? exp2_fast(m - mn) : 1.0f; // from -inf: 0
+                m = mn;
+                base = bn;
+                unbase = exp2_fast(-bn);
+                limit_w = far ? kKvNegInf : (mn - bn) + (kLift + kSlack);
+                if (i > 0 && __any_sync(kKvFull, out_down != 1.0f))
                 {
 #pragma unroll 1
                     for (int c = 0; c < D / 16; ++c)
@@ -558,18 +576,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                         tmem_ld_wait(o);
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            o[e] = __float_as_uint(__uint_as_float(o[e]) * down);
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) * out_down);
                         tmem_st16(o_addr + 16u * c, o);
                     }
                 }
             }
-            const float shift_m = m == kKvNegInf ? 0.0f : kLift - m;
-            // the exponent's product is not rounded where the maximum's was: beyond 2^20 that difference shows
-            const bool plain = whole && __all_sync(kKvFull, fabsf(m) < 1048576.0f);
-            if (plain)
-                weights(std::false_type{}, shift_m);
+            if (whole && __all_sync(kKvFull, fabsf(m) < kFar && fabsf(base) <= kTameBase))
+                weights(std::false_type{});
             else
-                weights(std::true_type{}, shift_m);
+                weights(std::true_type{});
             tmem_st_wait();
             fence_before();
             bar_arrive(bar(kPFull + tile));
@@ -583,10 +598,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         }
         const int r = w.r0 + tid;
         const bool live = r < w.r1;
-        const float lse2 = l == 0.0f ? kKvNegInf : m + log2f(l) - kLift;
-        float f = l == 0.0f ? 0.0f : vref / l;
+        const float lse2 = l == 0.0f ? kKvNegInf : m + log2f(l);
+        float f = l == 0.0f ? 0.0f : 1.0f / l;
         if (!ok)
             f = __int_as_float(0x7FC00000);
+        // unbase is apart from f: their product may leave the range of floats
         const int i = live ? r / G : 0, hd = (int)w.h * G + (live ? r % G : 0);
         const int item = (int)((w.b * p.c.hkv + w.h) * p.row_tiles + rt);
         float *part = p.part + (uint64_t)item * p.splits * kPromptRows * (D + 1);
@@ -621,8 +637,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                     float4 *dst = reinterpret_cast<float4 *>(part + ((uint64_t)w.split * kPromptRows + tid) * D + 32 * c);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        dst[e] = make_float4(__uint_as_float(x[4 * e]) * f, __uint_as_float(x[4 * e + 1]) * f,
-                                             __uint_as_float(x[4 * e + 2]) * f, __uint_as_float(x[4 * e + 3]) * f);
+                        dst[e] = make_float4(__uint_as_float(x[4 * e]) * f * unbase, __uint_as_float(x[4 * e + 1]) * f * unbase,
+                                             __uint_as_float(x[4 * e + 2]) * f * unbase,
+                                             __uint_as_float(x[4 * e + 3]) * f * unbase);
                 }
                 else if (live)
                 {
@@ -633,8 +650,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                         uint32_t y[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            y[k] = kv_pack<BF16>(__uint_as_float(x[8 * e + 2 * k]) * f,
-                                                 __uint_as_float(x[8 * e + 2 * k + 1]) * f);
+                            y[k] = kv_pack<BF16>(__uint_as_float(x[8 * e + 2 * k]) * f * unbase,
+                                                 __uint_as_float(x[8 * e + 2 * k + 1]) * f * unbase);
                         dst[e] = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
@@ -726,15 +743,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 }
             }
         };
-        auto convert = [&](uint8_t *tile, const uint4 (&r)[kPairs], uint32_t keep0, uint32_t keep1) {
+        auto convert = [&](uint8_t *tile, const uint4 (&r)[kPairs]) {
 #pragma unroll
             for (int it = 0; it < kPairs; ++it)
             {
                 const int pair = it * 4 + (lane >> 3), grp = pair / (D / 16), ch = pair % (D / 16);
                 const int row = cw * 32 + grp * 8 + (lane & 7);
-                const uint32_t keep = grp >= 2 ? keep1 : keep0, zero = 0x80808080u & ~keep;
-                const uint32_t u[4] = {(r[it].x & keep) | zero, (r[it].y & keep) | zero, (r[it].z & keep) | zero,
-                                       (r[it].w & keep) | zero};
+                const uint32_t u[4] = {r[it].x, r[it].y, r[it].z, r[it].w};
                 uint32_t y[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -770,22 +785,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 ok = bar_wait(bar(kKEmpty + st), par, gave_up);
             if (!__all_sync(kKvFull, ok))
                 break;
-            const float rel = fv > 0.0f ? fv / vref : 1.0f; // values of scale 0 become zeros and need no factor
             const bool held = (lane ? blk[1] : blk[0]) >= 0;
             if (lane < 2)
+            {
+                const float lg = log2f(fv);
+                const int pos = held ? w.base + i * kTok + cw * 32 + lane * 16 : kMaxPos;
                 s_f[(i % kFactorStages) * kGroups + cw * 2 + lane] =
-                    make_float4(fk, log2f(rel),
-                                __int_as_float(held ? w.base + i * kTok + cw * 32 + lane * 16 : kMaxPos), 1.0f / rel);
-            const uint32_t live[2] = {__shfl_sync(kKvFull, fv, 0) > 0.0f ? kKvFull : 0u,
-                                      __shfl_sync(kKvFull, fv, 1) > 0.0f ? kKvFull : 0u};
-            convert(smem + L::k + st * L::kTileBytes, rk, kKvFull, kKvFull);
+                    make_float4(fk, lg, __int_as_float(fabsf(lg) <= kTame ? pos : pos | (int)0x80000000), 1.0f / fv);
+            }
+            convert(smem + L::k + st * L::kTileBytes, rk);
             fence_smem();
             bar_arrive(bar(kKFull + st));
             if (i >= 2)
                 ok = bar_wait(bar(kVEmpty + st), par, gave_up);
             if (!__all_sync(kKvFull, ok))
                 break;
-            convert(smem + L::v + st * L::kTileBytes, rv, live[0], live[1]);
+            convert(smem + L::v + st * L::kTileBytes, rv);
             fence_smem();
             bar_arrive(bar(kVFull + st));
             // the next tile's loads come behind the fences, which would wait for them

@@ -339,6 +339,48 @@ def test_attention_factor_of_any_sign(dance_lib, rows, scale, dtype):
     check_lse(lse, want_lse, lse_err)
 
 
+def far_apart(power, where):
+    """Value scales 0.01, and 2^power times that in the blocks of the first sequence that `where` names."""
+    def make(w, pool):
+        s = np.full((pool, w.hkv), 0.01, np.float32)
+        s[w.table[0, where]] *= np.float32(2.0 ** power)
+        return s
+    return make
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS[2:])
+@pytest.mark.parametrize("dtype,power", [("float16", 15), ("float16", -16), ("bfloat16", 24), ("bfloat16", 34),
+                                         ("bfloat16", 90), ("bfloat16", -24), ("bfloat16", -100)])
+def test_attention_value_scales_far_apart(dance_lib, rows, dtype, power):
+    """One block's values are larger or smaller than the others' by a power of two; rows weigh it much and little."""
+    from dance_b200 import kvcache
+    w = Held([700, 65], [rows, 1], 1, 128, 64, dtype, seed=3, v_scale=far_apart(power, 4))
+    for size in (0.3, 2.0, 20.0):
+        q, qn = w.q(2, size)
+        out, lse = kvcache.attention(w.cache, w.batch, q, 0.1, return_lse=True)
+        want, want_lse, err, lse_err = w.attention(qn, 0.1)
+        check_out(out, want, err, dtype)
+        check_lse(lse, want_lse, lse_err)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS[2:])
+@pytest.mark.parametrize("dtype,power", [("float16", 15), ("bfloat16", 20), ("bfloat16", 34), ("bfloat16", 90)])
+def test_rows_do_not_depend_on_values_they_may_not_see(dance_lib, rows, dtype, power):
+    """The last block's values are far larger: rows before it give what they give where it is like the others."""
+    import torch
+    from dance_b200 import kvcache
+    outs, bs, last = [], 16, 2
+    lens = [19 * bs + last]
+    for p in (0, power):
+        w = Held(lens, [rows], 4, 96, bs, dtype, seed=5, v_scale=far_apart(p, -1))
+        q, qn = w.q(8)
+        outs.append(kvcache.attention(w.cache, w.batch, q, 0.1))
+        check_out(outs[-1], *w.attention(qn, 0.1)[::2], dtype)
+    assert torch.equal(outs[0][:rows - last], outs[1][:rows - last])
+
+
 # ------------------------------------------------------------------ workspaces
 def decode_step(tokens, seed=0, heads=8):
     """A call whose splits are joined through the workspace's counters."""
