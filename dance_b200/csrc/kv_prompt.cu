@@ -415,7 +415,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
     }
     __syncthreads();
     float m = kKvNegInf, l = 0.0f, base = kMostBase, unbase = 0.0f;
-    float limit_w = kKvNegInf; // of a logit plus log2 of its value scale, until base is set anew
     bool ok = true;
 
     if (warp < kSoftWarps)
@@ -450,7 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             loaded(x[1]);
             tmem_ld32(s_addr + 64u, x[2]);
             tmem_ld32(s_addr + 96u, x[3]);
-            float top = kKvNegInf, heavy = kKvNegInf; // largest logit; largest logit plus log2 of its value scale
+            float top = kKvNegInf, heavy = kKvNegInf; // largest logit; log2 of the largest p times value scale
+            float largest[kGroups];
             // the logits' factor is not negative and constant over 16 tokens
             auto maximum = [&](auto masked, int g0) {
 #pragma unroll
@@ -471,8 +471,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                     float y = m0 * (fg.x * rf);
                     if constexpr (masked)
                         y = m0 == kKvNegInf ? kKvNegInf : y;
+                    largest[g] = y;
                     top = fmaxf(top, y);
-                    heavy = fmaxf(heavy, y + fg.y);
+                    heavy = fmaxf(heavy, y - m + fg.y);
                 }
             };
             // Weights p = 2^(s - m), summed, and p times value scale times 2^base, the product's operand.  Plain tiles
@@ -495,18 +496,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                         {
-                            float2 z = fma2(make_float2(__uint_as_float(x[c][16 * u + 2 * e]),
-                                                        __uint_as_float(x[c][16 * u + 2 * e + 1])),
-                                            make_float2(kf, kf), make_float2(sm, sm));
+                            float2 z = make_float2(__uint_as_float(x[c][16 * u + 2 * e]),
+                                                   __uint_as_float(x[c][16 * u + 2 * e + 1]));
                             if constexpr (masked)
                             {
-                                // cut off what the exponent's unrounded product exceeds the maximum by; a logit
-                                // that is not a number stays one
-                                z.x = z.x > kSlack ? kSlack : z.x;
-                                z.y = z.y > kSlack ? kSlack : z.y;
-                                z.x = 2 * e < left ? z.x : kKvNegInf;
-                                z.y = 2 * e + 1 < left ? z.y : kKvNegInf;
+                                // products rounded as the maximum's is: none exceeds it, however far
+                                z.x = 2 * e < left ? __fadd_rn(__fmul_rn(z.x, kf), sm) : kKvNegInf;
+                                z.y = 2 * e + 1 < left ? __fadd_rn(__fmul_rn(z.y, kf), sm) : kKvNegInf;
                             }
+                            else
+                                z = fma2(z, make_float2(kf, kf), make_float2(sm, sm));
                             z.x = exp2_fast(z.x);
                             z.y = exp2_fast(z.y);
                             sum.x += z.x;
@@ -543,21 +542,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 }
                 fence_after();
             }
-            if (__any_sync(kKvFull, top > m + kSlack || heavy > limit_w))
+            if (__any_sync(kKvFull, top > m + kSlack || heavy + base > kLift + kSlack))
             {
                 // m: an integer, so that powers of two are all that sums and outputs are scaled by
                 const float mn = top > m + kSlack ? ceilf(top) : m; // from -inf: any maximum
-                const bool far = fabsf(mn) >= kFar && mn != kKvNegInf;
-                float need = heavy - mn; // log2 of the largest p times value scale
-                if (__any_sync(kKvFull, far))
-                {
-                    // where the sum's rounding hides the scale: the tile's largest, with the most that p can be
-                    float most = kKvNegInf;
-#pragma unroll 1
-                    for (int g = 0; g < kGroups; ++g)
-                        most = fmaxf(most, f[g].y);
-                    need = far ? kSlack + most : need;
-                }
+                float need = kKvNegInf;
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g)
+                    need = fmaxf(need, largest[g] - mn + f[g].y);
                 const float keep = fminf(base + (mn - m), kMostBase); // leaves O as it is; from -inf: kMostBase
                 const float bn = need + keep > kLift + kSlack ? fmaxf(floorf(kLift - need), -kMostBase) : keep;
                 const float out_down = mn != m || bn != base ? exp2_fast((m - mn) + (bn - base)) : 1.0f;
@@ -565,7 +557,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 m = mn;
                 base = bn;
                 unbase = exp2_fast(-bn);
-                limit_w = far ? kKvNegInf : (mn - bn) + (kLift + kSlack);
                 if (i > 0 && __any_sync(kKvFull, out_down != 1.0f))
                 {
 #pragma unroll 1

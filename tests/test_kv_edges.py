@@ -381,6 +381,34 @@ def test_rows_do_not_depend_on_values_they_may_not_see(dance_lib, rows, dtype, p
     assert torch.equal(outs[0][:rows - last], outs[1][:rows - last])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ROWS[2:])
+@pytest.mark.parametrize("size", (1e6, 1e7, 3e7, 1e8, 3e8, 1e12, 1e30))
+def test_attention_far_logits(dance_lib, rows, size):
+    """Logits of a million and more: one token takes all where it leads by more than the logits' error; its values are
+    the output."""
+    from dance_b200 import kvcache
+    w = Held([700], [rows], 1, 128, 64, "bfloat16", seed=rows, v_scale=far_apart(20, 4))
+    q, qn = w.q(2, size)
+    out, lse = kvcache.attention(w.cache, w.batch, q, 0.1, return_lse=True)
+    got, clear = out.double().cpu().numpy(), 0
+    assert np.isfinite(got).all() and np.isfinite(lse.cpu().numpy()).all()
+    at = w.table[0]
+    k = (w.k[at, 0] * w.ks[at, 0].astype(np.float64)[:, None, None]).reshape(-1, 128)
+    v = (w.v[at, 0] * w.vs[at, 0].astype(np.float64)[:, None, None]).reshape(-1, 128)
+    for r in range(rows):
+        n = 700 - rows + r + 1
+        for g in range(2):
+            x = 0.1 * (k[:n] @ qn[r, g])
+            first, second = np.argsort(-x)[:2]
+            error = 2 * (128 + 8) * 2.0 ** -23 * 0.1 * (np.abs(k[:n]) @ np.abs(qn[r, g])).max()
+            if x[first] - x[second] > 2 * error + 60:
+                clear += 1
+                want = v[first]
+                assert (np.abs(got[r, g] - want) <= (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -19) * np.abs(want)).all()
+    assert clear > rows
+
+
 # ------------------------------------------------------------------ workspaces
 def decode_step(tokens, seed=0, heads=8):
     """A call whose splits are joined through the workspace's counters."""
