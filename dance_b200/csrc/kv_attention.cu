@@ -5,16 +5,20 @@
 // Mathematics.  With codes k = kc - 128, v = vc - 128 (integers of 8 bits,
 // exact in half precision) and block scales sk, sv:
 //   s_j = scale * sk * (q . k_j),   o = sum_j p_j sv v_j / sum_j p_j,
-//   p_j = 2^(s_j log2 e - m), m the running maximum of the row.
+//   p_j = 2^(s_j log2 e - m), m the running maximum of the row, a whole number
+//   that stays until it is exceeded by 6 (8 in prompt_kernel).
 // Scales are constant in a block, so they stay out of the matrix products: sk
 // multiplies the logits, sv the weights.
 //
 // Roundings.  q enters as halves after an exact division by a power of two
 // per row (bfloat16 has fewer bits than half; what underflows is below 2^-38
 // of the row's largest channel).  The weights enter the second product as
-// halves of 2^14 p_j sv / (largest sv so far): 11 bits, and a weight counts
-// down to 2^-38 of the row's largest.  Products are summed in float, as are m,
-// the sum of the weights (taken before rounding) and the output.
+// halves of p_j sv 2^base, 11 bits.  base is a row's own, set so that its
+// largest p_j sv becomes 2^8 to 2^9 here (2^6 to 2^7 in prompt_kernel), and set
+// anew before one passes 2^15: a weight has its 11 bits down to 2^-22 (2^-20)
+// of the largest and is lost below 2^-33 (2^-31).  It comes from the tokens
+// that the row sees alone.  Products are summed in float, as are the p_j, before
+// rounding, and the output.
 //
 // Two kernels: rows_kernel here for the few rows of decode steps, drafts and
 // chosen blocks, where the cache's bytes bound the call, and prompt_kernel
@@ -44,7 +48,10 @@ constexpr int kTile = 32;       // tokens of a warp's tile
 // warps hide what a third tile would: 171 against 172 us for a step of 96 sequences, 68 against 80 for the sparse one.
 constexpr int kStages = 2;
 constexpr int kEntries = 256;   // cache blocks looked up at once
-constexpr float kBoost = 14.0f; // log2 of what a weight of 1 is as a half
+constexpr float kLift = 9.0f;   // log2 of a row's largest weight when its base is set
+constexpr float kSlack = 6.0f;  // how far maximum and weights may rise before they are set anew
+constexpr float kMostBase = 126.0f; // bases whose power of two, and its inverse, are normal numbers
+constexpr float kMostTimes = 8.507059e37f; // 2^126
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src)
 {
@@ -141,6 +148,13 @@ template <int D>
 constexpr int rows_smem()
 {
     return ring_bytes<D>() + kEntries * 20;
+}
+
+// Thread blocks an SM: by shared memory, and by registers for 16 rows.
+template <int D, int NT>
+constexpr int rows_blocks()
+{
+    return D == 128 ? 4 - NT : 5 - NT;
 }
 
 // The blocks that any of ntok adjacent query tokens chose, each once, with a
@@ -246,7 +260,7 @@ __device__ int unite_lists(const AttnParams &p, const KvSeq &s, uint32_t h, int 
 // and then the splits, are joined at the end, the splits by the block that
 // finishes last, in their order.
 template <int D, int NT, bool SPARSE, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
+__global__ void __launch_bounds__(kWarps * 32, rows_blocks<D, NT>()) rows_kernel(AttnParams p)
 {
     extern __shared__ __align__(128) uint8_t smem[];
     constexpr int kRows = 8 * NT, kSteps = D / 16, kV = D / 8;
@@ -339,12 +353,14 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
     };
 
     float o[kSteps][NT][4];
-    float m[NT][2], l[NT][2], vref = 0.0f;
+    float m[NT][2], l[NT][2], base[NT][2], times[NT][2]; // times: 2^base
 #pragma unroll
     for (int j = 0; j < NT; ++j)
     {
         m[j][0] = m[j][1] = kKvNegInf;
         l[j][0] = l[j][1] = 0.0f;
+        base[j][0] = base[j][1] = kMostBase;
+        times[j][0] = times[j][1] = kMostTimes;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
             o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
@@ -443,6 +459,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
                 continue;
             }
             const float kf[2] = {s_kf[ea], s_kf[eb]}, vs[2] = {s_vs[ea], s_vs[eb]};
+            const float ve[2] = {scale_exponent(vs[0]), scale_exponent(vs[1])};
 
             // ---- logits
             float sc[2][NT][4];
@@ -474,14 +491,13 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
                 whole &= (chosen[0] & chosen[1]) == (1u << ntok) - 1u;
             }
             bool up = false;
-            float mn[NT][2];
+            float most[NT][2][2]; // the lane's largest logits
 #pragma unroll
             for (int j = 0; j < NT; ++j)
             {
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
                 {
-                    float top = m[j][k];
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt)
                     {
@@ -493,22 +509,15 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
                             if (!whole && (pos[mt] + g + 8 * u >= limit[j][k] || (SPARSE && !(chosen[mt] & chose[j][k]))))
                                 x = kKvNegInf;
                             sc[mt][j][2 * u + k] = x;
-                            top = fmaxf(top, x);
                         }
+                        most[j][k][mt] = fmaxf(sc[mt][j][k], sc[mt][j][2 + k]);
                     }
-                    top = fmaxf(top, __shfl_xor_sync(kKvFull, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(kKvFull, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(kKvFull, top, 16));
-                    mn[j][k] = top;
-                    up |= top > m[j][k];
+                    const float a = most[j][k][0] - m[j][k], b = most[j][k][1] - m[j][k];
+                    up |= fmaxf(a, b) > kSlack || fmaxf(a + ve[0], b + ve[1]) + base[j][k] > kLift + kSlack;
                 }
             }
-            const float vmax = fmaxf(vs[0], vs[1]);
-            if (__any_sync(kKvFull, up) || vmax > vref)
+            if (__any_sync(kKvFull, up))
             {
-                const float vn = fmaxf(vref, vmax);
-                const float vdown = vn > 0.0f ? __fdividef(vref, vn) : 1.0f;
-                vref = vn;
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
                 {
@@ -516,10 +525,25 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
                     {
-                        down[k] = mn[j][k] == kKvNegInf ? 1.0f : exp2_fast(m[j][k] - mn[j][k]);
-                        l[j][k] *= down[k];
-                        m[j][k] = mn[j][k];
-                        down[k] *= vdown;
+                        float top = fmaxf(most[j][k][0], most[j][k][1]);
+                        top = fmaxf(top, __shfl_xor_sync(kKvFull, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(kKvFull, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(kKvFull, top, 16));
+                        // whole numbers: powers of two are all that sums and outputs are scaled by
+                        const float mn = top > m[j][k] + kSlack ? ceilf(top) : m[j][k];
+                        float need = fmaxf(most[j][k][0] - mn + ve[0], most[j][k][1] - mn + ve[1]);
+                        need = fmaxf(need, __shfl_xor_sync(kKvFull, need, 4));
+                        need = fmaxf(need, __shfl_xor_sync(kKvFull, need, 8));
+                        need = fmaxf(need, __shfl_xor_sync(kKvFull, need, 16));
+                        const float rise = mn - m[j][k]; // from -inf: inf, or not a number where it stays
+                        const float keep = fminf(base[j][k] + rise, kMostBase); // leaves the output as it is
+                        const float bn = need + keep > kLift + kSlack ? fmaxf(floorf(kLift - need), -kMostBase) : keep;
+                        const bool none = mn == kKvNegInf;
+                        l[j][k] *= none ? 1.0f : exp2_fast(-rise);
+                        down[k] = none ? 1.0f : exp2_fast(bn - base[j][k] - rise);
+                        m[j][k] = mn;
+                        base[j][k] = bn;
+                        times[j][k] = exp2_fast(bn);
                     }
 #pragma unroll
                     for (int i = 0; i < kSteps; ++i)
@@ -533,24 +557,24 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
             }
 
             // ---- weights and their product with the values
-            const float vinv = vref > 0.0f ? __fdividef(1.0f, vref) : 0.0f;
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
             {
-                const float vf = vs[mt] * vinv;
                 uint32_t pb[NT][2];
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
                 {
-                    const float m0 = m[j][0] == kKvNegInf ? 0.0f : m[j][0] - kBoost;
-                    const float m1 = m[j][1] == kKvNegInf ? 0.0f : m[j][1] - kBoost;
+                    const float m0 = m[j][0] == kKvNegInf ? 0.0f : m[j][0];
+                    const float m1 = m[j][1] == kKvNegInf ? 0.0f : m[j][1];
+                    // a block that the row does not see may have any scale: 0 times it has to be 0
+                    const float f0 = fminf(vs[mt] * times[j][0], kMostTimes), f1 = fminf(vs[mt] * times[j][1], kMostTimes);
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
                     {
                         const float p0 = exp2_fast(sc[mt][j][2 * u] - m0), p1 = exp2_fast(sc[mt][j][2 * u + 1] - m1);
                         l[j][0] += p0;
                         l[j][1] += p1;
-                        pb[j][u] = transpose8(kv_pack<false>(p0 * vf, p1 * vf));
+                        pb[j][u] = transpose8(kv_pack<false>(p0 * f0, p1 * f1));
                     }
                 }
                 uint32_t v0[D / 32], v1[D / 32], v8[D / 32], v9[D / 32];
@@ -616,11 +640,11 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
             float top = kKvNegInf;
             for (int w = 0; w < kWarps; ++w)
                 top = fmaxf(top, s_m[w * kRows + r]);
-            const float f = (m[j][k] == kKvNegInf ? 0.0f : exp2_fast(m[j][k] - top)) * vref;
+            const float f = m[j][k] == kKvNegInf ? 0.0f : exp2_fast(m[j][k] - top), unbase = exp2_fast(-base[j][k]);
             float *dst = s_o + (warp * kRows + r) * D + g * kV;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
-                *reinterpret_cast<float2 *>(dst + 2 * i) = make_float2(o[i][j][k] * f, o[i][j][2 + k] * f);
+                *reinterpret_cast<float2 *>(dst + 2 * i) = make_float2(o[i][j][k] * f * unbase, o[i][j][2 + k] * f * unbase);
         }
     __syncthreads();
     const int item = (int)((SPARSE ? ((b * p.groups + (uint32_t)tg) * p.c.hkv + h) : (b * p.c.hkv + h)) *
@@ -638,7 +662,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(AttnParams p)
         for (int w = 0; w < kWarps; ++w)
             sum += s_m[w * kRows + r] == kKvNegInf ? s_l[w * kRows + r]
                                                    : exp2_fast(s_m[w * kRows + r] - top) * s_l[w * kRows + r];
-        const float lse2 = sum == 0.0f ? kKvNegInf : top + log2f(sum) - kBoost;
+        const float lse2 = sum == 0.0f ? kKvNegInf : top + log2f(sum);
         s_all[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
         if (nsplits > 1)
             part_lse[split * kRows + r] = lse2;
@@ -796,8 +820,7 @@ AttnPlan plan_attention(const DanceKvCache &c, const DanceKvBatch &b, uint32_t h
         // whole waves of equal blocks.  Sequences of unknown lengths up to max_len: the work spread over the slots,
         // and the last block's own time.  (Steps of 96 sequences up to 8192 tokens, 8 heads: 1 split 175 us, 2 171,
         // 4 165.  24 of up to 6000, 4 heads: 4 splits 26.7, 7 23.5, 13 33.)
-        // Blocks an SM: by shared memory, and by registers for 16 rows.
-        const uint32_t per_sm = a.nt == 1 ? (c.head_dim == 128 ? 3u : 4u) : (c.head_dim == 128 ? 2u : 3u);
+        const uint32_t per_sm = c.head_dim == 128 ? 4u - a.nt : 5u - a.nt; // rows_blocks()
         const uint64_t slots = (uint64_t)kSms * per_sm;
         const uint64_t most = std::min<uint64_t>((tokens + 255) / 256, kMostSplits);
         const uint64_t fixed = 384ull * a.nt * 128 / c.head_dim;

@@ -72,5 +72,7 @@ __device__ __forceinline__ int row_shift(float amax)
     return (ex == 255 || amax == 0.0f) ? 0 : min(126, 127 + 13 - ex);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// The least whole number above log2 of a value scale; -126 for 0.
+__device__ __forceinline__ float scale_exponent(float s) { return (float)((int)(__float_as_uint(s) >> 23) - 126); }
 
 } // namespace dance

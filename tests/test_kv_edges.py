@@ -349,7 +349,7 @@ def far_apart(power, where):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", ROWS[2:])
+@pytest.mark.parametrize("rows", ROWS)
 @pytest.mark.parametrize("dtype,power", [("float16", 15), ("float16", -16), ("bfloat16", 24), ("bfloat16", 34),
                                          ("bfloat16", 90), ("bfloat16", -24), ("bfloat16", -100)])
 def test_attention_value_scales_far_apart(dance_lib, rows, dtype, power):
@@ -365,7 +365,7 @@ def test_attention_value_scales_far_apart(dance_lib, rows, dtype, power):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", ROWS[2:])
+@pytest.mark.parametrize("rows", ROWS[1:])
 @pytest.mark.parametrize("dtype,power", [("float16", 15), ("bfloat16", 20), ("bfloat16", 34), ("bfloat16", 90)])
 def test_rows_do_not_depend_on_values_they_may_not_see(dance_lib, rows, dtype, power):
     """The last block's values are far larger: rows before it give what they give where it is like the others."""
@@ -379,10 +379,16 @@ def test_rows_do_not_depend_on_values_they_may_not_see(dance_lib, rows, dtype, p
         outs.append(kvcache.attention(w.cache, w.batch, q, 0.1))
         check_out(outs[-1], *w.attention(qn, 0.1)[::2], dtype)
     assert torch.equal(outs[0][:rows - last], outs[1][:rows - last])
+    # adjacent rows that choose apart: only some of them the large block
+    blocks = np.full((rows, 4, 3), -1)
+    blocks[:, :, 0] = np.arange(rows)[:, None] % 3
+    blocks[1::2, :, 1] = 19
+    out = kvcache.sparse_attention(w.cache, w.batch, q, int32(blocks), 0.1)
+    check_out(out, *w.attention(qn, 0.1, blocks)[::2], dtype)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", ROWS[2:])
+@pytest.mark.parametrize("rows", ROWS)
 @pytest.mark.parametrize("size", (1e6, 1e7, 3e7, 1e8, 3e8, 1e12, 1e30))
 def test_attention_far_logits(dance_lib, rows, size):
     """Logits of a million and more: one token takes all where it leads by more than the logits' error; its values are
