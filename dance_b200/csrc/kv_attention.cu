@@ -14,9 +14,9 @@
 // per row (bfloat16 has fewer bits than half; what underflows is below 2^-38
 // of the row's largest channel).  The weights enter the second product as
 // halves of p_j sv 2^base, 11 bits.  base is a row's own, set so that its
-// largest p_j sv becomes 2^8 to 2^9 here (2^6 to 2^7 in prompt_kernel), and set
-// anew before one passes 2^15: a weight has its 11 bits down to 2^-22 (2^-20)
-// of the largest and is lost below 2^-33 (2^-31).  It comes from the tokens
+// largest p_j sv becomes 2^7 to 2^9 here (2^6 to 2^7 in prompt_kernel), and set
+// anew before one passes 2^15: a weight has its 11 bits down to 2^-21 (2^-20)
+// of the largest and is lost below 2^-32 (2^-31).  It comes from the tokens
 // that the row sees alone.  Products are summed in float, as are the p_j, before
 // rounding, and the output.
 //

@@ -127,7 +127,7 @@ __device__ __forceinline__ float kv_step_of(float amax)
     const float s = __fmul_rn(amax, 1.0f / 127.0f);
     return s < kKvTiny ? 0.0f : s;
 }
-__device__ __forceinline__ float kv_inverse(float s) { return s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f; }
+__device__ __forceinline__ float kv_inverse(float s) { return s >= kKvTiny ? __fdiv_rn(1.0f, s) : 0.0f; }
 __device__ __forceinline__ int kv_code(float x, float inv)
 {
     // min and max of NaN and a number give the number: NaN is told apart first

@@ -448,8 +448,8 @@ DANCE_API int dance_partition_buckets(const uint32_t *d_assign, uint64_t num_poi
  * Block b, head h, token t, channel d of the keys is the byte
  *   d_k[b * k_block_stride + (h * block_tokens + t) * head_dim + d],
  * likewise the values; a code c stands for (c - 128) * scale with one float
- * scale, not negative, per block and head (d_k_scale, d_v_scale: num_blocks x
- * kv_heads).
+ * scale, finite and not negative, per block and head (d_k_scale, d_v_scale:
+ * num_blocks x kv_heads); new rows in a block of a scale below 2^-126 become 0.
  * d_k_bounds (num_blocks x kv_heads x 2 x head_dim) holds the smallest and
  * the largest key code of every channel over the block's tokens.  head_dim
  * is 64, 96 or 128; pointers and block strides are multiples of 16 bytes. */

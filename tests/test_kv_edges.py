@@ -388,6 +388,26 @@ def test_rows_do_not_depend_on_values_they_may_not_see(dance_lib, rows, dtype, p
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", (1, 40))
+def test_scales_without_an_inverse(dance_lib, rows):
+    """Blocks whose scales have no finite inverse: new rows become 0, attention stays finite."""
+    import torch
+    from dance_b200 import kvcache
+    w = Held([320], [rows], 1, 64, 32, "bfloat16", seed=2, k_scale=far_apart(-126, 3), v_scale=far_apart(-126, 3))
+    assert 0 < w.ks.min() < 2.0 ** -126
+    q, qn = w.q(2)
+    out, lse = kvcache.attention(w.cache, w.batch, q, 0.1, return_lse=True)
+    want, want_lse, err, lse_err = w.attention(qn, 0.1)
+    check_out(out, want, err, "bfloat16")
+    check_lse(lse, want_lse, lse_err)
+    x = torch.zeros((8, 1, 64), dtype=torch.bfloat16, device="cuda")
+    x[1::2] = 2.0 ** -130
+    kvcache.append(w.cache, batch_of(w.table, [3 * 32 + 10], [8]), x, x)
+    for t in (w.cache.k, w.cache.v):
+        assert (t[int(w.table[0, 3]), 0, 2:10] == 128).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", ROWS)
 @pytest.mark.parametrize("size", (1e6, 1e7, 3e7, 1e8, 3e8, 1e12, 1e30))
 def test_attention_far_logits(dance_lib, rows, size):
