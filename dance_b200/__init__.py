@@ -227,6 +227,7 @@ SIGNATURES = {
     "dance_kv_attention": (_I, [_P, _P, _P, _U32, _F, _P, _P, _P, _U64, _P]),
     "dance_kv_select_blocks": (_I, [_P, _P, _P, _U32, _U32, _U32, _U32, _P, _P, _U64, _P]),
     "dance_kv_sparse_attention": (_I, [_P, _P, _P, _U32, _P, _U32, _F, _P, _P, _P, _U64, _P]),
+    "dance_kv_status": (_I, []),
     "dance_kv_workspace_bytes": (_U64, [_P, _P, _U32, _U32, _U32]),
     "dance_stitched_build_sharded": (_I, [_P, _I, _P, _U32, _U32, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32, _P,
                                           _U32, _P, _P, _U64, _P, _P]),

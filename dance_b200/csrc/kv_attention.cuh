@@ -29,6 +29,7 @@ struct AttnParams
     float *lse;
     uint32_t *counters;
     float *part; // partial outputs, then partial log-sums
+    long long wait_clocks; // limit of a wait on a barrier (prompt kernel)
 };
 
 // How a call is cut: row tiles, splits, workspace.
@@ -44,7 +45,7 @@ struct AttnPlan
 // Rows of a tile of the kernel of many rows (kv_prompt.cu).
 constexpr uint32_t kPromptRows = 256;
 constexpr uint32_t kPromptTokens = 128;
-int launch_prompt(const AttnParams &p, uint32_t head_dim, bool bf16, uint32_t blocks_x, cudaStream_t st);
+int launch_prompt(AttnParams &p, uint32_t head_dim, bool bf16, uint32_t blocks_x, cudaStream_t st);
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 

@@ -46,9 +46,11 @@
 // keep, were no faster: 783 us for the call above, against 774.)
 //
 // Every wait on a barrier is bounded.  A block that gives up counts itself in
-// g_kv_prompt_timeouts, and its rows read as not-a-number.
+// g_kv_prompt_timeouts, which dance_kv_status reads, and its rows read as
+// not-a-number.
 #include <cuda_runtime.h>
 
+#include <cstdlib>
 #include <type_traits>
 
 #include "kv_attention.cuh"
@@ -127,15 +129,21 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
                  : "memory");
     return ok != 0;
 }
-// Bounded wait; false (with *gave_up set for the whole block) when it ran out.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *gave_up)
+// Bounded wait; false (with *gave_up set for the whole block) when it ran out.  The last try comes after the time: a
+// block that was switched out for longer finds its barrier ready.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, long long clocks, volatile int *gave_up)
 {
     if (bar_try(bar, parity))
         return true;
     const long long begin = clock64();
-    while (clock64() - begin < kWaitClocks && !*gave_up)
+    for (;;)
+    {
+        const bool over = clock64() - begin >= clocks || *gave_up;
         if (bar_try(bar, parity))
             return true;
+        if (over)
+            break;
+    }
     *gave_up = 1;
     return false;
 }
@@ -362,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         bar_init(bar(kSFree), 128);
         bar_init(bar(kDrain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-        *gave_up = 0;
+        *gave_up = p.wait_clocks > 0 ? 0 : 1; // a limit of nothing has run out
     }
     fence_before();
     __syncthreads();
@@ -428,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         const int tile_lo = min(w.s.first + (w.r0 + 128 * tile) / G + 1, w.s.len); // least that a row of the tile sees
         for (int i = 0; i < (tile == 0 || two ? w.tiles : 0); ++i)
         {
-            ok = bar_wait(bar(kSFull + tile), (uint32_t)i & 1u, gave_up);
+            ok = bar_wait(bar(kSFull + tile), (uint32_t)i & 1u, p.wait_clocks, gave_up);
             if (!__all_sync(kKvFull, ok))
             {
                 ok = false;
@@ -534,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             // the product before is done with O and with the place of the weights
             if (i > 0)
             {
-                ok = bar_wait(bar(kODone + tile), (uint32_t)(i - 1) & 1u, gave_up);
+                ok = bar_wait(bar(kODone + tile), (uint32_t)(i - 1) & 1u, p.wait_clocks, gave_up);
                 if (!__all_sync(kKvFull, ok))
                 {
                     ok = false;
@@ -583,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
         // ------------------------------------------------ out
         if (w.tiles > 0 && ok && (tile == 0 || two))
         {
-            ok = bar_wait(bar(kODone + tile), (uint32_t)(w.tiles - 1) & 1u, gave_up);
+            ok = bar_wait(bar(kODone + tile), (uint32_t)(w.tiles - 1) & 1u, p.wait_clocks, gave_up);
             ok = __all_sync(kKvFull, ok);
             fence_after();
         }
@@ -773,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             const int st = i & 1;
             const uint32_t par = (uint32_t)((i >> 1) + 1) & 1u; // of the stage's release before this use
             if (i >= 2)
-                ok = bar_wait(bar(kKEmpty + st), par, gave_up);
+                ok = bar_wait(bar(kKEmpty + st), par, p.wait_clocks, gave_up);
             if (!__all_sync(kKvFull, ok))
                 break;
             const bool held = (lane ? blk[1] : blk[0]) >= 0;
@@ -788,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
             fence_smem();
             bar_arrive(bar(kKFull + st));
             if (i >= 2)
-                ok = bar_wait(bar(kVEmpty + st), par, gave_up);
+                ok = bar_wait(bar(kVEmpty + st), par, p.wait_clocks, gave_up);
             if (!__all_sync(kKvFull, ok))
                 break;
             convert(smem + L::v + st * L::kTileBytes, rv);
@@ -807,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
     {
         // ------------------------------------------------ matrix instructions
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kMmaRegs));
-        if (warp == kMmaWarp)
+        if (warp == kMmaWarp && !__any_sync(kKvFull, *gave_up))
         {
             // The whole warp walks the loop and one lane issues: with every address the same in all lanes by
             // construction (reductions and votes), the operands stay in uniform registers.
@@ -823,9 +831,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(AttnParams p)
                 if (__all_sync(kKvFull, bar_try(bar(which), parity)))
                     return true;
                 const long long begin = clock64();
-                while (__all_sync(kKvFull, clock64() - begin < kWaitClocks && !*gave_up))
+                for (;;)
+                {
+                    const bool over = clock64() - begin >= p.wait_clocks || *gave_up;
                     if (__all_sync(kKvFull, bar_try(bar(which), parity)))
                         return true;
+                    if (__any_sync(kKvFull, over))
+                        break;
+                }
                 *gave_up = 1;
                 return false;
             };
@@ -901,8 +914,11 @@ int launch(const AttnParams &p, uint32_t blocks_x, cudaStream_t st)
 
 } // namespace
 
-int launch_prompt(const AttnParams &p, uint32_t head_dim, bool bf16, uint32_t blocks_x, cudaStream_t st)
+int launch_prompt(AttnParams &p, uint32_t head_dim, bool bf16, uint32_t blocks_x, cudaStream_t st)
 {
+    const char *limit = std::getenv("DANCE_KV_WAIT_CLOCKS");
+    p.wait_clocks = limit ? std::atoll(limit) : kWaitClocks;
+    p.wait_clocks = p.wait_clocks < 0 || p.wait_clocks > kWaitClocks ? kWaitClocks : p.wait_clocks;
     switch (head_dim)
     {
     case 64:
@@ -915,3 +931,19 @@ int launch_prompt(const AttnParams &p, uint32_t head_dim, bool bf16, uint32_t bl
 }
 
 } // namespace dance
+
+using namespace dance;
+
+extern "C" int dance_kv_status(void)
+{
+    unsigned int t = 0;
+    DANCE_CUDA(cudaDeviceSynchronize());
+    DANCE_CUDA(cudaMemcpyFromSymbol(&t, g_kv_prompt_timeouts, sizeof(t)));
+    if (t)
+    {
+        const unsigned int z = 0;
+        DANCE_CUDA(cudaMemcpyToSymbol(g_kv_prompt_timeouts, &z, sizeof(z)));
+        return fail(-4, "key/value attention: %u blocks gave up waiting", t);
+    }
+    return 0;
+}

@@ -17,7 +17,7 @@ block score, or a graph search over the keys, picked:
 
 All tensors are CUDA tensors of one device; the calls take ``stream`` (None:
 torch's current stream), on which they run and allocate, neither synchronise nor copy to the host, and may be
-captured in a CUDA graph.  The kernels are those of ``dance_kv_*`` in
+captured in a CUDA graph; ``status`` tells whether they finished.  The kernels are those of ``dance_kv_*`` in
 include/dance_b200.h, where the formulas and the layouts stand.
 """
 from __future__ import annotations
@@ -28,7 +28,8 @@ from ctypes import addressof as _address
 
 from . import DANCE_BF16, DANCE_F16, DANCE_F32, DanceKvBatch, DanceKvCache, DanceKvRows, check, load
 
-__all__ = ["KVCache", "KVBatch", "KVWorkspace", "append", "read", "attention", "select_blocks", "sparse_attention"]
+__all__ = ["KVCache", "KVBatch", "KVWorkspace", "append", "read", "attention", "select_blocks", "sparse_attention",
+           "status"]
 
 HEAD_DIMS = (64, 96, 128)
 BLOCK_TOKENS = (16, 32, 64, 128)
@@ -387,3 +388,9 @@ def select_blocks(cache: KVCache, batch: KVBatch, q, select: int, *, first_block
     if rc:
         check(rc, "dance_kv_select_blocks")
     return out
+
+
+def status() -> None:
+    """Waits for the current device and raises DanceError where blocks of an attention call gave up waiting and left
+    not-a-number in their rows.  To be called where results are handed on."""
+    check(load().dance_kv_status(), "dance_kv_status")

@@ -558,6 +558,11 @@ DANCE_API int dance_kv_sparse_attention(const DanceKvCache *cache, const DanceKv
                                         uint32_t num_heads, const int32_t *d_blocks, uint32_t select, float scale,
                                         void *d_out, float *d_lse, void *d_workspace, uint64_t workspace_bytes,
                                         void *stream);
+/* Whether every attention call on the current device since the last call of
+ * this function finished its work: 0, or -4 where blocks of it gave up waiting
+ * (about a second for one of their own steps) and left not-a-number in their
+ * rows.  Synchronises with the device; not for use in a stream capture. */
+DANCE_API int dance_kv_status(void);
 /* Workspace bytes that the attention (select = 0), or the selection and the
  * block-sparse attention (select > 0), of such a call can need. */
 DANCE_API uint64_t dance_kv_workspace_bytes(const DanceKvCache *cache, const DanceKvBatch *batch, uint32_t rows,

@@ -581,3 +581,29 @@ def test_attention_on_a_second_device(dance_lib):
                 q, _ = w.q(2)
                 outs.append(kvcache.attention(w.cache, w.batch, q).cpu())
         assert torch.equal(*outs)
+
+
+# ------------------------------------------------------------------ waits that run out
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", (700, 30000))
+def test_waits_that_run_out_are_told(dance_lib, monkeypatch, tokens):
+    """With a limit of nothing the blocks give up and say so; the calls after it are whole again."""
+    import torch
+    from dance_b200 import DanceError, kvcache
+    cache, _, _ = decode_step(tokens)
+    batch = batch_of([list(range(cache.num_blocks))], [tokens], [300])
+    q = torch.randn((300, 8, 64), device="cuda").half()
+    ws = kvcache.KVWorkspace()
+    want, lse = kvcache.attention(cache, batch, q, return_lse=True, workspace=ws)
+    kvcache.status()
+    assert torch.isfinite(want).all()
+    monkeypatch.setenv("DANCE_KV_WAIT_CLOCKS", "0")
+    out = kvcache.attention(cache, batch, q, workspace=ws)
+    with pytest.raises(DanceError, match="gave up waiting"):
+        kvcache.status()
+    assert torch.isnan(out).any()
+    kvcache.status()  # told once
+    monkeypatch.delenv("DANCE_KV_WAIT_CLOCKS")
+    again, lse_again = kvcache.attention(cache, batch, q, return_lse=True, workspace=ws)
+    kvcache.status()
+    assert torch.equal(again, want) and torch.equal(lse_again, lse)
