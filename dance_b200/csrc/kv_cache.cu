@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(D / 8 * kTokenGroups, IT <= 2 ? 1536 / (D / 8 
     __shared__ uint2 lo_s[kTokenGroups][kD8], hi_s[kTokenGroups][kD8];
     const uint32_t b = blockIdx.y, h = blockIdx.x % p.c.hkv; // heads of a token side by side
     const KvSeq s = kv_seq(p.c, b, p.rows);
-    const int start = max(s.first, 0), end = s.first + s.rows;
+    const int start = max(s.first, 0), end = min(s.first + s.rows, s.len);
     const int page = start / kBs + (int)(blockIdx.x / p.c.hkv);
     const int base = page * kBs;
     const int lo = max(start, base), hi = min(end, base + kBs);
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(256) read_kernel(KvView c, uint32_t rows, void
     {
         const uint32_t d8 = (uint32_t)(e % kD8), rh = (uint32_t)(e / kD8), h = rh % c.hkv, i = rh / c.hkv;
         const int pos = s.first + (int)i;
-        const int blk = pos >= 0 ? kv_block(c, b, pos >> c.shift) : -1;
+        const int blk = pos >= 0 && pos < s.len ? kv_block(c, b, pos >> c.shift) : -1;
         const uint64_t si = (uint64_t)max(blk, 0) * c.hkv + h;
         const uint64_t in = (((uint64_t)h << c.shift) + ((uint32_t)pos & mask)) * D + d8 * 8;
         const uint64_t out = ((uint64_t)(s.row0 + i) * c.hkv + h) * D + d8 * 8;

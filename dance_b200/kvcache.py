@@ -107,7 +107,9 @@ class KVBatch:
     the call's new rows; row_offsets: int32 (batch + 1,), the rows of sequence
     b being row_offsets[b] .. row_offsets[b + 1], its last row at its last
     token.  max_rows and max_len: bounds of rows and tokens of a sequence, known
-    on the host.  The tensors may be updated in place between calls.
+    on the host; what lies beyond is not visited.  Rows that belong to no
+    sequence, or lie beyond max_rows, are not written: in a new output they hold
+    anything.  The tensors may be updated in place between calls.
     """
 
     def __init__(self, block_table, seq_lens, row_offsets, max_rows: int, max_len: int):

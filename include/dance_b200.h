@@ -476,7 +476,9 @@ typedef struct DanceKvCache
  * table_width); entries outside [0, num_blocks) hold no tokens: writes to
  * them are dropped, reads see nothing there.  max_rows and max_len bound the
  * rows and the length of every sequence (they size the launch; rows and
- * tokens beyond them are not visited).  batch <= 65535. */
+ * tokens beyond them are not visited: not written, read as 0, not attended
+ * to).  Rows of an output that belong to no sequence, or lie beyond max_rows,
+ * are left as they are.  batch <= 65535. */
 typedef struct DanceKvBatch
 {
     const int32_t *d_block_table;

@@ -104,6 +104,29 @@ def test_append_codes_are_those_of_the_step(dance_lib, dim, bs, dtype):
     assert np.array_equal(b[:, :, 0], want.min(2)) and np.array_equal(b[:, :, 1], want.max(2))
 
 
+@pytest.mark.gpu
+def test_tokens_beyond_the_largest_length_are_not_visited(dance_lib):
+    """Appended rows beyond max_len are dropped, read as 0; rows of no sequence keep what their place held."""
+    import torch
+    from dance_b200 import kvcache
+    cache = kvcache.KVCache.create(6, 1, 64, 16)
+    x = torch.randn((40, 1, 64), device="cuda").half() + 3
+    batch = batch_of([[0, 1, 2, 3]], [50], [40], max_len=33)
+    kvcache.append(cache, batch, x, x)
+    k = cache.k[:, 0].cpu().numpy()
+    assert (k[0, :10] == 128).all() and (k[0, 10:] != 128).any(1).all() and (k[1] != 128).any(1).all()
+    assert (k[2, 0] != 128).any() and (k[2, 1:] == 128).all() and (k[3:] == 128).all()
+    assert (cache.k_scale[3:] == 0).all()
+    got, _ = kvcache.read(cache, batch, 40, torch.float32)
+    assert (got[23:] == 0).all() and (got[:23] != 0).any(2).all()
+    assert torch.allclose(got[:23], x[:23].float(), atol=0.05)
+    # rows 1 and 2 of four are a sequence's
+    some = kvcache.KVBatch(int32([[0, 1, 2, 3]]), int32([30]), int32([1, 3]), 2, 30)
+    out = torch.full((4, 2, 64), 7.0, device="cuda").half()
+    kvcache.attention(cache, some, torch.randn((4, 2, 64), device="cuda").half(), out=out)
+    assert (out[0] == 7).all() and (out[3] == 7).all() and (out[1:3] != 7).all()
+
+
 # ------------------------------------------------------------------ selection
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -181,6 +204,14 @@ def test_append_equals_the_twin(dance_lib, twin, dim, bs, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_append_of_odd_values_equals_the_twin(dance_lib, twin, dtype):
     test_kvcache.test_append_odd_values(dance_lib, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("check", [
+    test_kvcache.test_append_strided_and_unaligned, test_kvcache.test_append_outside_the_table_and_before_the_start])
+def test_append_beside_the_twin(dance_lib, twin, check):
+    for _ in range(4):
+        check(dance_lib)
 
 
 @pytest.mark.gpu
