@@ -466,6 +466,81 @@ def test_attention_far_logits(dance_lib, rows, size):
     assert clear > rows
 
 
+# ------------------------------------------------------------------ rows that share their chosen blocks
+def lists(kind, rows, heads, select, pages, rng):
+    """Block lists of adjacent rows: alike, apart, out of order, with repeats, with places past the end."""
+    out = np.full((rows, heads, select), -1)
+    common = rng.permutation(pages)[:select]
+    for r in range(rows):
+        for h in range(heads):
+            mine = rng.permutation(pages)[:select]
+            take = common if kind == "same" else np.where(rng.random(len(mine)) < 0.5, common[:len(mine)], mine)
+            got = np.unique(take)
+            if kind == "short":
+                got = got[:rng.integers(0, len(got) + 1)]
+            if kind == "unsorted":
+                got = rng.permutation(got)
+            if kind == "twice":
+                got = np.concatenate([got, got])[:select]
+            if kind == "outside":
+                got = np.concatenate([got[:select - 2], [pages + 3, 1 << 30]])
+            out[r, h, :len(got)] = got
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ("same", "apart", "short", "unsorted", "twice", "outside"))
+@pytest.mark.parametrize("G,dim,bs,select,rows", [
+    (1, 64, 16, 7, 301), (2, 128, 64, 11, 299), (3, 96, 16, 5, 333), (4, 64, 32, 60, 301), (1, 128, 128, 32, 300)])
+def test_sparse_attention_of_adjacent_rows(dance_lib, kind, G, dim, bs, select, rows):
+    """Hundreds of rows over four heads: a thread block takes several tokens (8 / G, a last group of fewer)."""
+    from dance_b200 import kvcache
+    pages = max(select + 3, 9)
+    w = Held([pages * bs - 3], [rows], 4, dim, bs, "float16", seed=G + select)
+    table = w.table.copy()
+    table[0, 1] = -1 if G % 2 else 10 ** 6  # a block that holds nothing
+    w.batch = batch_of(table, w.lens, w.rows)
+    blocks = lists(kind, rows, 4, select, pages, w.rng)
+    q, qn = w.q(4 * G)
+    out, lse = kvcache.sparse_attention(w.cache, w.batch, q, int32(blocks), 0.1, return_lse=True)
+    blocks[blocks == 1] = -1
+    want, want_lse, err, lse_err = w.attention(qn, 0.1, blocks)
+    check_out(out, want, err, "float16")
+    check_lse(lse, want_lse, lse_err)
+    assert kind != "short" or np.isinf(want_lse).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,G,blocks", [(1, 2, 9729), (3, 1, 20001), (2, 3, 9728)])
+def test_selection_of_more_blocks_than_shared_memory_holds(dance_lib, rows, G, blocks):
+    """Scores read from memory in every cut; and the most that shared memory holds."""
+    import torch
+    from dance_b200 import kvcache
+    rng = np.random.default_rng(blocks)
+    low = rng.integers(-127, 20, (blocks, 64))
+    high = low + rng.integers(0, 107, (blocks, 64))
+    ks = rng.choice(np.array([0.01, 0.02, 0.03], np.float32), (blocks, 1))
+    code = torch.full((blocks, 1, 16, 64), 128, dtype=torch.uint8, device="cuda")
+    bounds = torch.tensor(np.stack((low, high), 1)[:, None] + 128, device="cuda").to(torch.uint8)
+    scale = torch.tensor(ks, device="cuda")
+    cache = kvcache.KVCache(code, code, scale, scale, bounds)
+    q = torch.tensor(rng.normal(size=(rows, G, 64)), device="cuda").half()
+    batch = batch_of([np.arange(blocks)], [16 * blocks], [rows])
+    for select, first, last in ((1, 0, 0), (64, 1, 1), (4096, 3, 5)):
+        got = kvcache.select_blocks(cache, batch, q, select, first_blocks=first, last_blocks=last).cpu().numpy()
+        for r in range(rows):
+            score = np.full(blocks, -np.inf, np.float32)
+            for g in range(G):
+                x = q[r, g].float().cpu().numpy()
+                s = step_of(x)
+                c = np.rint(x * (np.float32(1) / s)).astype(np.int64)
+                score = np.maximum(score, np.maximum(c * low, c * high).sum(1).astype(np.float32) * s)
+            score = score * ks[:, 0]
+            score[:first] = np.inf
+            score[blocks - last:] = np.inf
+            assert np.array_equal(got[r, 0], np.sort(np.lexsort((np.arange(blocks), -score))[:select]))
+
+
 # ------------------------------------------------------------------ workspaces
 def decode_step(tokens, seed=0, heads=8):
     """A call whose splits are joined through the workspace's counters."""
