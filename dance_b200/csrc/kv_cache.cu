@@ -382,9 +382,9 @@ extern "C" int dance_kv_append(const DanceKvCache *cache, const DanceKvBatch *ba
 {
     if (int rc = kv_check(cache, batch))
         return rc;
-    if (int rc = kv_check_rows(k, cache->head_dim, cache->kv_heads, "k"))
+    if (int rc = kv_check_rows(k, "k"))
         return rc;
-    if (int rc = kv_check_rows(v, cache->head_dim, cache->kv_heads, "v"))
+    if (int rc = kv_check_rows(v, "v"))
         return rc;
     if (k->rows != v->rows || k->dtype != v->dtype)
         return fail(-1, "keys (%u rows, dtype %d) and values (%u rows, dtype %d) differ", k->rows, k->dtype, v->rows,

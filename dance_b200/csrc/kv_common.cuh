@@ -172,7 +172,7 @@ inline int kv_check(const DanceKvCache *c, const DanceKvBatch *b)
     return 0;
 }
 
-inline int kv_check_rows(const DanceKvRows *r, uint32_t head_dim, uint32_t heads, const char *name)
+inline int kv_check_rows(const DanceKvRows *r, const char *name)
 {
     if (!r)
         return fail(-1, "null rows %s", name);
@@ -184,8 +184,6 @@ inline int kv_check_rows(const DanceKvRows *r, uint32_t head_dim, uint32_t heads
         return fail(-1, "null or misaligned rows %s", name);
     if (r->rows > 0x7FFFFFFFu)
         return fail(-1, "%s has too many rows", name);
-    (void)head_dim;
-    (void)heads;
     return 0;
 }
 

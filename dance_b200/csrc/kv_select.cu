@@ -680,7 +680,7 @@ extern "C" int dance_kv_select_blocks(const DanceKvCache *cache, const DanceKvBa
 {
     if (int rc = kv_check(cache, batch))
         return rc;
-    if (int rc = kv_check_rows(q, cache->head_dim, num_heads, "q"))
+    if (int rc = kv_check_rows(q, "q"))
         return rc;
     if (num_heads == 0 || num_heads % cache->kv_heads || num_heads > 65536)
         return fail(-1, "num_heads %u must be a multiple of kv_heads %u", num_heads, cache->kv_heads);
