@@ -24,13 +24,16 @@
 // chosen blocks, where the cache's bytes bound the call, and prompt_kernel
 // (kv_prompt.cu) from 33 rows of a sequence and key/value head, where the
 // products do.  Measured (rows_kernel): one token over 2.2M tokens, 64 heads on
-// 8 of 128: 710 to 740 us, 6.1 to 6.3 TB/s, 0.93 to 0.97 of the measured copy
-// rate; one token of each of 96 sequences up to 8192 tokens, 32 heads on 8: 165
-// to 176 us, 5.3 to 5.7 TB/s; 64 chosen blocks of 64 tokens of each of 32
-// sequences: 62 us, 4.3 TB/s (short blocks' start and end); 700 rows of 24
-// heads on 8 of 96 over 48 chosen blocks of 32: 217 us, 1.65 GB out of L2, bound
-// by instructions (conversion of codes) and latency; 24 sequences' drafts of up
-// to 5 tokens over up to 6000: 27 us, latency.
+// 8 of 128: 755 to 770 us, 5.9 to 6.0 TB/s, 0.90 of the measured copy rate; one
+// token of each of 96 sequences up to 8192 tokens, 32 heads on 8: 179 to 181 us,
+// 5.2 TB/s; 64 chosen blocks of 64 tokens of each of 32 sequences: 62 us, 4.3
+// TB/s (short blocks' start and end); 700 rows of 24 heads on 8 of 96 over 48
+// chosen blocks of 32: 215 us, 1.65 GB out of L2, bound by instructions
+// (conversion of codes) and latency; 24 sequences' drafts of up to 5 tokens over
+// up to 6000: 29 us, latency.  Maximum and base that move only when they have to
+// save the exchange between a row's eight lanes in most tiles, about what the
+// row's own base costs: with one maximum of the value scales for all rows,
+// taken and exchanged in every tile, the five took 748, 178, 62, 217 and 28.6.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -45,7 +48,8 @@ namespace
 constexpr int kWarps = 4;
 constexpr int kTile = 32;       // tokens of a warp's tile
 // Tiles of a warp in flight or in use.  Two leave room for three blocks an SM at 128 channels and four below, whose
-// warps hide what a third tile would: 171 against 172 us for a step of 96 sequences, 68 against 80 for the sparse one.
+// warps hide what a third tile would (with the kernel of that time, 171 against 172 us for a step of 96 sequences, 68
+// against 80 for the sparse one).
 constexpr int kStages = 2;
 constexpr int kEntries = 256;   // cache blocks looked up at once
 constexpr float kLift = 9.0f;   // log2 of a row's largest weight when its base is set

@@ -74,6 +74,10 @@ __device__ __forceinline__ int row_shift(float amax)
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // The least whole number above log2 of a value scale; -126 for 0.
-__device__ __forceinline__ float scale_exponent(float s) { return (float)((int)(__float_as_uint(s) >> 23) - 126); }
+__device__ __forceinline__ float scale_exponent(float s)
+{
+    // the exponent's bits as the last of 2^23 + e, exactly
+    return __uint_as_float((__float_as_uint(s) >> 23) | 0x4B000000u) - (8388608.0f + 126.0f);
+}
 
 } // namespace dance

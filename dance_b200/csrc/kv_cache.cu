@@ -13,9 +13,10 @@
 // minima and maxima in registers and one reduction over 16 groups.
 //
 // Both kernels move each byte once.  Measured: 17106 tokens x 8 heads of 96
-// channels in blocks of 32, f16: append 34 us (79 MB, 2.3 TB/s; instructions
-// bound it, about 29 per element with their block's share of setup and
-// reductions), read 19 us (79 MB, 4.1 TB/s).  One token of each of 64 sequences
+// channels in blocks of 32, f16: append 35 us (79 MB, 2.3 TB/s; instructions
+// bound it, about 31 per element with their block's share of setup and
+// reductions, 74 % of the issue slots), read 20 us (79 MB, 4.0 TB/s, 77 % of the
+// issue slots).  One token of each of 64 sequences
 // x 8 heads of 128: append 6 to 9 us, read 5, latency.  Taking the keys and the
 // values of a block together, magnitudes as packed integers and codes by adding
 // a constant brought the append from 46 us.

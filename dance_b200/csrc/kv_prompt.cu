@@ -13,7 +13,7 @@
 // columns of S, 2 x 64 of P, 2 x head_dim of O, full at 128 channels.
 //
 // Measured on 2594 rows x 32 heads over 16000 and 7100 tokens of 128 channels:
-// 0.77 ms, 0.73 PFLOP/s (0.44 of the measured matrix rate).  A token tile takes
+// 0.78 ms, 0.72 PFLOP/s (0.44 of the measured matrix rate).  A token tile takes
 // about 4900 clocks where the tensor core works 2100: what bounds it are the
 // softmax threads' 3200 clocks for a tile (two warps a scheduler, the
 // exponentials half of it) and the turning of codes into halves; tensor core,
@@ -43,7 +43,7 @@
 // tokens that the row sees alone, however far apart the blocks' value scales lie;
 // m and base are whole numbers, which sums and outputs are scaled by exactly.
 // (Weights taken relative to the split's largest value scale, with no base to
-// keep, were no faster: 783 us for the call above, against 774.)
+// keep, were no faster: 783 us for the call above, against 779.)
 //
 // Every wait on a barrier is bounded.  A block that gives up counts itself in
 // g_kv_prompt_timeouts, which dance_kv_status reads, and its rows read as

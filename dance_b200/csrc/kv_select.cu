@@ -13,8 +13,9 @@
 // Floor: the bounds' 2 * head_dim bytes of every (block, head), once.  Measured:
 // 32 sequences of up to 1875 blocks, 8 heads of 128 channels (54.7 MB): 28 us,
 // scores 19 (2.9 TB/s), choice 6, a launch between them.  700 rows of one
-// sequence, 24 heads of 96, 2049 blocks: 94 us, scores 46, choice 47; both
-// kernels wait on latency there, not on the 4 us that bytes and products need.
+// sequence, 24 heads of 96, 2049 blocks: 94 us, scores 46, choice 47;
+// latency and instructions bound both there (54 and 76 % of the issue slots), not
+// the 4 us that bytes and products need.
 //
 // scores_kernel writes the float scores of (row, head, block) from integer
 // matrix instructions, choose_kernel finds each (row, head)'s threshold in
