@@ -771,7 +771,11 @@ __global__ void __launch_bounds__(kWarps * 32, rows_blocks<D, NT>()) rows_kernel
 constexpr uint32_t kSms = 148;
 constexpr uint64_t kMostSplits = 480; // their weights are joined in the ring's shared memory
 static_assert((kMostSplits + 8) * 16 * 4 <= rows_smem<64>(), "weights of the splits");
-constexpr uint64_t kPromptLeast = 32;      // rows of a sequence and key/value head from which it is used
+// The prompt kernel takes over above this many rows (query tokens x query heads) of a sequence and key/value head.  8
+// key/value heads of 128, prompt kernel against rows_kernel: 40 rows of 24 sequences of 6000 tokens 225 and 188 us, of
+// one of 60000 91 and 80; 64 rows of 8 sequences of 8000 96 and 128, 128 rows 107 and 226; 256 rows of 2 of 16000 117
+// and 215.  They meet between 40 and 64 rows.
+constexpr uint64_t kPromptLeast = 32;
 
 AttnPlan plan_attention(const DanceKvCache &c, const DanceKvBatch &b, uint32_t heads, uint32_t select)
 {
@@ -823,7 +827,7 @@ AttnPlan plan_attention(const DanceKvCache &c, const DanceKvBatch &b, uint32_t h
         // A block's start and end count like 384 tokens of 128 channels and 8 rows, and so does joining.  One sequence, or lists of one length:
         // whole waves of equal blocks.  Sequences of unknown lengths up to max_len: the work spread over the slots,
         // and the last block's own time.  (Steps of 96 sequences up to 8192 tokens, 8 heads: 1 split 175 us, 2 171,
-        // 4 165.  24 of up to 6000, 4 heads: 4 splits 26.7, 7 23.5, 13 33.)
+        // 4 165.  24 of up to 6000, 4 heads: 4 splits 26.7, 7 23.5, 13 33; of these the rule can take 4.)
         const uint32_t per_sm = c.head_dim == 128 ? 4u - a.nt : 5u - a.nt; // rows_blocks()
         const uint64_t slots = (uint64_t)kSms * per_sm;
         const uint64_t most = std::min<uint64_t>((tokens + 255) / 256, kMostSplits);

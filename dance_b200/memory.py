@@ -26,7 +26,8 @@ MOST_FOUND = 256  # the search's list
 
 
 class KeyIndex:
-    """Vamana graph over the keys of one sequence and key/value head."""
+    """Vamana graph over the keys of one sequence and key/value head, those of its building: tokens appended later are
+    chosen with the last block only, which blocks_of_tokens always takes."""
 
     def __init__(self, keys, R: int = 32, L: int = 64, C: int = 64, steps: int = 32):
         """keys: CUDA tensor (tokens, head_dim), as kvcache.read gives them."""
